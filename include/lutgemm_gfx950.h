@@ -668,6 +668,136 @@ int lutgemm_describe_attention_plan(int batch, int heads, int kv_heads, int head
  * pointers 16-byte aligned. */
 int lutgemm_decode_silu_mul_f16(const void *gate, const void *up, void *out, size_t count, void *stream);
 
+/*
+ * ---- attention over a cache held in 4 bits (no counterpart in the reference) ---------------------------------------------------
+ * A cache of keys and values in groups of 32 numbers along the head, 4 bits each, with a scale and a minimum per group in
+ * fp16: 5 bits a number.  A held value is the fp16 number fp16(minimum + scale * code).
+ *   layout: [batch][kv_heads][ceil(max_positions / 32)] blocks of 40 * head_dim bytes, 32 positions each; with G = head_dim / 32
+ *     uint32 key codes    [32 positions][4 quads][G]          dimensions 32 t + 8 quad + e of group t
+ *     fp16   key scales   [32 positions][G][scale, minimum]
+ *     uint32 value codes  [4 quads][16 columns][2 G]          dimension 16 t + column of positions 4 quad + e (e < 4) and
+ *                                                             16 + 4 quad + e - 4 (e >= 4)
+ *     fp16   value scales [G][scale, minimum][4 quads][8]     the positions in the same order
+ *   a word holds eight codes e = 0..7: the even ones in its low half from bit 0 up, the odd ones in its high half.
+ *   A group x[32] is held as minimum = min x, scale = fp16(fp32((max x - min x) / 15)), code = (x - minimum) / scale rounded
+ *   to the nearest of 0..15, halves to even (0 where the scale is 0).  Numbers beyond +-60000, infinities among them, are held
+ *   as +-60000 and NaN as 0: a cache holds finite numbers only, and what is written by other means must keep to that.
+ *   16-byte aligned; it needs no initial contents.  lutgemm_q4_cache_bytes: its size, 0 for sizes that are not taken
+ *   (head_dim a multiple of 32, at most 256; 1 <= max_positions <= 2^20).
+ *
+ * One call takes `tokens` new tokens of every sequence: a single one, a few, or a prompt.
+ *   q, k, v      fp16 [batch][tokens][heads (kv_heads) * head_dim], strides in elements: *_stride[0] between sequences, [1]
+ *                between tokens, multiples of 8, 0 or more; 16-byte aligned.  heads a multiple of kv_heads, at most 4096
+ *   cos, sin     fp16 [max_positions][head_dim], the two halves of a row equal (rotate-half convention); 16-byte aligned
+ *   start        int64 [batch], device: the position of a sequence's first new token
+ *   counts       NULL (all `tokens`), or int32 [batch], device: how many of its tokens are there
+ *   out          fp16 [batch][tokens][heads * head_dim], contiguous, 16-byte aligned
+ *   k_held, v_held  NULL, or fp16 [batch][tokens][kv_heads * head_dim], contiguous, 16-byte aligned: the values that the
+ *                cache now holds for the new tokens
+ * Token i of a sequence stands at position start + i.  Its key is rotated (rounded to fp16) and appended with its value, and
+ * its query, rotated likewise, attends to the held values of positions 0 .. start + i, its own among them:
+ * softmax(q k^T / sqrt(head_dim)) v, sums in fp32.  Tokens beyond a sequence's count, tokens at positions outside the cache,
+ * and all of a sequence whose start is negative (an idle slot) are passed over: nothing is appended, and their rows of out,
+ * k_held and v_held are zeros.  Positions that are not attended to have no influence, whatever the cache holds there; a
+ * sequence's earlier positions are the caller's to have filled.  out, k_held, v_held and the cache may not overlap anything.
+ *
+ * `workspace`: lutgemm_q4_attention_workspace bytes (0: none needed; the size does not depend on what start and counts
+ * hold), 16-byte aligned, of any contents, in use until the call's work is done.  Nothing is allocated, the launches
+ * depend on the sizes alone, so a captured call can be replayed for other positions.
+ */
+typedef struct lutgemm_q4_attention {
+    void *cache;
+    const void *q, *k, *v, *cos_table, *sin_table;
+    const int64_t *start;
+    const int32_t *counts;
+    void *out, *k_held, *v_held;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+    int batch, tokens, heads, kv_heads, head_dim, max_positions;
+} lutgemm_q4_attention;
+
+size_t lutgemm_q4_cache_bytes(int batch, int kv_heads, int max_positions, int head_dim);
+size_t lutgemm_q4_attention_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_positions);
+int lutgemm_q4_attention_f16(const lutgemm_q4_attention *call, void *workspace, size_t workspace_bytes, void *stream);
+
+/* How such a call would be launched (host arithmetic); returns what the call would return for these sizes. */
+typedef struct lutgemm_q4_attention_plan {
+    int launches;        /* of kernels */
+    int fused;           /* 1: new tokens are appended by the attention launch itself */
+    int rows_per_wave;   /* (token, query head) rows of a kv head that a wave takes, a multiple of 16 */
+    int row_tiles;       /* tiles of rows per (sequence, kv head): a wave's, or a workgroup's where its waves take different rows */
+    int rows_apart;      /* 1: the waves of a workgroup take different rows, 0: different positions */
+    int splits;          /* workgroups that share the positions of a tile */
+    int workgroups;      /* of the attention launch */
+    int threads;
+} lutgemm_q4_attention_plan;
+int lutgemm_describe_q4_attention_plan(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_positions,
+                                       lutgemm_q4_attention_plan *plan);
+
+/*
+ * ---- choosing the next token (no counterpart in the reference, which takes the most likely one) ---------------------------------
+ * One token per row of logits, from given random numbers.  Per row, with l the logits and m the largest:
+ *   weight     w = exp((l - m) / temperature); a logit of +inf counts as infinitely above every other one, -inf and NaN as
+ *              weight 0 whatever the temperature
+ *   order      larger logits first, equal ones by index
+ *   top_k      the first top_k tokens of that order                              (<= 0: all)
+ *   top_p      of those, the shortest run whose weights come to at least top_p times theirs, one token at least (>= 1: all)
+ *   min_p      of those, the tokens with w >= min_p; the largest always stay     (<= 0: all)
+ *   drawn      the first of those left whose running sum of weights exceeds uniform times their sum
+ *   logprob    ln of its share of that sum
+ * temperature <= 0: the first token of the order, logprob 0.  A row without weight (all -inf or NaN): id -1, logprob -inf.
+ * A parameter that is NaN counts as off (temperature as 0, uniform as 0).  uniform is taken into [0, 1); what rounding leaves
+ * behind the last sum is the last token left.
+ * Weights are formed in 64 bits, held to 2^-43 of the largest (2^-52 up to 2048 tokens) and added as whole numbers: the same result
+ * whatever the order, and the one that the formulas give in 64 bits but for numbers that lie within about 2^-40 of a border.
+ *   logits     [rows][vocab] of logits_type (LUTGEMM_TYPE_*), row_stride elements between rows, aligned to their own size
+ *   temperature, top_p, min_p, uniform  float [rows], top_k int32 [rows], device; all but uniform may be NULL (1, off)
+ *   ids        int64 [rows]; logprob  NULL, or float [rows]
+ *   1 <= rows <= 65535, 1 <= vocab <= 2^20
+ * `workspace`: lutgemm_sampling_workspace bytes, 16-byte aligned, of any contents, in use until the call's work is done.
+ */
+typedef struct lutgemm_sampling {
+    const void *logits;
+    int64_t row_stride;
+    int logits_type, rows, vocab;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p, *uniform;
+    int64_t *ids;
+    float *logprob;
+} lutgemm_sampling;
+
+size_t lutgemm_sampling_workspace(int rows, int vocab);
+int lutgemm_sample_tokens(const lutgemm_sampling *call, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * ---- low-rank adapters beside a shared linear layer (no counterpart in the reference) -------------------------------------------
+ * Every row takes the adapter that its id names, or none: a = ids[m],
+ *   out[m][n] = fp16(base[m][n] + scale[a] * sum_r up[a][n][r] * h[r]),   h[r] = sum_k down[a][r][k] * x[m][k]
+ * with h and the sums in fp32; out[m] = base[m] where a is not in 0 .. adapters - 1.
+ *   x [M][K], base [M][N], out [M][N] fp16, rows x_stride, base_stride, out_stride elements apart (x_stride a multiple of 8, the others
+ *   of 4); x 16-byte aligned, base and out 8-byte aligned; out may be base itself, with its stride
+ *   ids int32 [M], device;  down fp16 [adapters][rank][K], up fp16 [adapters][N][rank], 16-byte aligned;  scale float
+ *   [adapters], or NULL (1)
+ *   K % 32 == 0, N % 4 == 0, rank % 8 == 0, 8 <= rank <= 256 (adapters of other or unlike ranks are filled up with zeros),
+ *   1 <= M <= 65535, 1 <= adapters <= 65535
+ * Several layers of one call (projections that share their input, or do not) share its launches: 1 <= count <=
+ * LUTGEMM_MAX_GROUP.  What one of them writes may not overlap what another reads or writes.
+ * `workspace`: lutgemm_adapters_workspace bytes (0 for arguments that are refused), 16-byte aligned, of any contents, in use until
+ * the call's work is done.
+ */
+typedef struct lutgemm_adapters {
+    const void *x_f16, *base_f16;
+    void *out_f16;
+    const int32_t *ids;
+    const void *down_f16, *up_f16;
+    const float *scale;
+    int64_t x_stride, base_stride, out_stride;
+    int M, N, K, rank, adapters;
+} lutgemm_adapters;
+
+size_t lutgemm_adapters_workspace(int count, const lutgemm_adapters *problems);
+int lutgemm_adapters_f16(int count, const lutgemm_adapters *problems, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -301,6 +301,264 @@ PyObject *linear_forward_py(PyObject *, PyObject *const *args, Py_ssize_t n)
 PyMethodDef linear_forward_def = {"linear_forward", (PyCFunction)(void (*)(void))linear_forward_py, METH_FASTCALL,
                                   "LutLinear.forward in one call"};
 
+// ---- a served token's other operators (no counterpart in the reference) -------------------------------------
+const at::Tensor *optional_tensor(PyObject *o, const char *name)
+{
+    if (o == Py_None) return nullptr;
+    TORCH_CHECK_TYPE(THPVariable_Check(o), name, ": expected a tensor or None, got ", Py_TYPE(o)->tp_name);
+    return &THPVariable_Unpack(o);
+}
+
+const at::Tensor &required_tensor(PyObject *o, const char *name)
+{
+    TORCH_CHECK_TYPE(THPVariable_Check(o), name, ": expected a tensor, got ", Py_TYPE(o)->tp_name);
+    return THPVariable_Unpack(o);
+}
+
+void check_like(const at::Tensor &t, const char *name, const at::Device &device, c10::ScalarType dtype)
+{
+    TORCH_CHECK(t.device() == device, name, " must be on ", device, ", is on ", t.device());
+    TORCH_CHECK(t.scalar_type() == dtype, name, " must be ", c10::toString(dtype), ", is ", c10::toString(t.scalar_type()));
+}
+
+void check_vector(const at::Tensor &t, const char *name, const at::Device &device, c10::ScalarType dtype, int64_t numel)
+{
+    check_like(t, name, device, dtype);
+    TORCH_CHECK(t.is_contiguous() && t.numel() == numel, name, " must hold ", numel, " contiguous values, has shape ", t.sizes());
+}
+
+void refuse_gradient(std::initializer_list<const at::Tensor *> ts, const char *fn)
+{
+    if (!at::GradMode::is_enabled()) return;
+    for (const at::Tensor *t : ts)
+        TORCH_CHECK(!t || !t->requires_grad(), fn, " has no gradient: call it under torch.no_grad() or detach its operands");
+}
+
+at::Tensor workspace_of(size_t bytes, const at::Device &device)
+{
+    if (bytes == 0) return {};
+    return at::Tensor(at::detail::empty_cuda({(int64_t)bytes}, at::kByte, device, c10::nullopt));
+}
+
+bool rows_are(const at::Tensor &t, int64_t multiple, uintptr_t bytes)
+{
+    if ((uintptr_t)t.const_data_ptr() % bytes != 0 || (t.size(-1) > 1 && t.stride(-1) != 1)) return false;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && (t.stride(i) < 0 || t.stride(i) % multiple != 0)) return false;
+    return true;
+}
+
+// q4_attend(cache, q, k, v, cos, sin, start, counts, out, held, max_positions) -> out, or (out, k_held, v_held)
+PyObject *q4_attend_py(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 11, "q4_attend takes 11 arguments, got ", n);
+    const at::Tensor &cache = required_tensor(args[0], "cache"), &cos = required_tensor(args[4], "cos"),
+                     &sin = required_tensor(args[5], "sin"), &start = required_tensor(args[6], "start");
+    at::Tensor q = required_tensor(args[1], "q"), k = required_tensor(args[2], "k"), v = required_tensor(args[3], "v");
+    const at::Tensor *counts = optional_tensor(args[7], "counts"), *given = optional_tensor(args[8], "out");
+    const bool held = PyObject_IsTrue(args[9]) == 1;
+    const int64_t max_positions = PyLong_AsLongLong(args[10]);
+    if (max_positions == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK(cache.is_cuda(), "the cache must be a GPU tensor");
+    const auto device = cache.device();
+    TORCH_CHECK(cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.is_contiguous(), "the cache must be a contiguous uint8 [batch, kv_heads, blocks, bytes]");
+    const int64_t B = cache.size(0), KV = cache.size(1), hd = cache.size(3) / 40;
+    TORCH_CHECK(max_positions >= 1 && max_positions <= 1 << 20 && hd >= 32 && hd <= 256 && B <= 65535 && KV <= 4096 &&
+                    (size_t)cache.numel() == lutgemm_q4_cache_bytes((int)B, (int)KV, (int)max_positions, (int)hd) && cache.numel() > 0,
+                "the cache has the wrong size for ", max_positions, " positions: ", cache.sizes());
+    refuse_gradient({&q, &k, &v, &cos, &sin}, "attend");
+    const bool flat = q.dim() == 2;
+    TORCH_CHECK(q.dim() == 3 || flat, "q must be [batch, tokens, heads * head_dim] or [batch, heads * head_dim], is ", q.sizes());
+    const int64_t T = flat ? 1 : q.size(1), H = q.size(-1) / hd;
+    TORCH_CHECK(T >= 1 && T <= 65536, "1 to 65536 new tokens a sequence, got ", T);
+    TORCH_CHECK(H >= KV && H <= 4096 && H % KV == 0 && q.size(-1) == H * hd, "q must hold a multiple of ", KV, " heads of ", hd, ", has ", q.size(-1), " values a token");
+    auto row = [&](at::Tensor &t, const char *name, int64_t heads) {
+        check_like(t, name, device, at::kHalf);
+        TORCH_CHECK(t.dim() == q.dim() && t.size(0) == B && (flat || t.size(1) == T) && t.size(-1) == heads * hd, name, " must be ",
+                    B, " x ", T, " x ", heads * hd, ", is ", t.sizes());
+        if (!rows_are(t, 8, 16)) t = t.clone(at::MemoryFormat::Contiguous);
+    };
+    row(k, "k", KV);
+    row(v, "v", KV);
+    row(q, "q", H);
+    for (const at::Tensor *t : {&cos, &sin}) {
+        check_like(*t, "cos and sin", device, at::kHalf);
+        TORCH_CHECK(t->dim() == 2 && t->size(0) >= max_positions && t->size(1) == hd && t->is_contiguous(), "cos and sin must be contiguous [max_positions, head_dim], are ", t->sizes());
+    }
+    check_vector(start, "start", device, at::kLong, B);
+    if (counts) check_vector(*counts, "counts", device, at::kInt, B);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
+    auto allocate = [&](int64_t heads) {
+        const int64_t three[] = {B, T, heads * hd}, two[] = {B, heads * hd};
+        return at::Tensor(at::detail::empty_cuda(flat ? at::IntArrayRef(two) : at::IntArrayRef(three), at::kHalf, device, c10::nullopt));
+    };
+    if (given) {
+        check_like(*given, "out", device, at::kHalf);
+        TORCH_CHECK(given->numel() == B * T * H * hd && given->is_contiguous(), "out must be ", B, " x ", T, " x ", H * hd, " contiguous values");
+    }
+    at::Tensor out = given ? *given : allocate(H), k_held, v_held;
+    if (held) {
+        k_held = allocate(KV);
+        v_held = allocate(KV);
+    }
+    lutgemm_q4_attention c{};
+    c.cache = cache.data_ptr();
+    c.q = q.const_data_ptr();
+    c.k = k.const_data_ptr();
+    c.v = v.const_data_ptr();
+    c.cos_table = cos.const_data_ptr();
+    c.sin_table = sin.const_data_ptr();
+    c.start = (const int64_t *)start.const_data_ptr();
+    c.counts = counts ? (const int32_t *)counts->const_data_ptr() : nullptr;
+    c.out = out.data_ptr();
+    c.k_held = held ? k_held.data_ptr() : nullptr;
+    c.v_held = held ? v_held.data_ptr() : nullptr;
+    auto strides = [&](int64_t *s, const at::Tensor &t) {
+        s[0] = B > 1 ? t.stride(0) : 0;
+        s[1] = T > 1 ? t.stride(1) : 0;
+    };
+    strides(c.q_stride, q);
+    strides(c.k_stride, k);
+    strides(c.v_stride, v);
+    c.batch = (int)B;
+    c.tokens = (int)T;
+    c.heads = (int)H;
+    c.kv_heads = (int)KV;
+    c.head_dim = (int)hd;
+    c.max_positions = (int)max_positions;
+    const size_t bytes = lutgemm_q4_attention_workspace(c.batch, c.tokens, c.heads, c.kv_heads, c.head_dim, c.max_positions);
+    const at::Tensor workspace = workspace_of(bytes, device);
+    raise_on_error(lutgemm_q4_attention_f16(&c, bytes ? workspace.data_ptr() : nullptr, bytes,
+                                            c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream()), "attend");
+    if (!held) return THPVariable_Wrap(out);
+    return PyTuple_Pack(3, py::reinterpret_steal<py::object>(THPVariable_Wrap(out)).ptr(), py::reinterpret_steal<py::object>(THPVariable_Wrap(k_held)).ptr(),
+                        py::reinterpret_steal<py::object>(THPVariable_Wrap(v_held)).ptr());
+    END_HANDLE_TH_ERRORS
+}
+
+// sample_tokens(logits, uniform, temperature, top_k, top_p, min_p) -> (ids, logprob)
+PyObject *sample_tokens_py(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 6, "sample_tokens takes 6 arguments, got ", n);
+    at::Tensor logits = required_tensor(args[0], "logits");
+    const at::Tensor &uniform = required_tensor(args[1], "uniform");
+    const at::Tensor *temperature = optional_tensor(args[2], "temperature"), *top_k = optional_tensor(args[3], "top_k"),
+                     *top_p = optional_tensor(args[4], "top_p"), *min_p = optional_tensor(args[5], "min_p");
+    TORCH_CHECK(logits.is_cuda(), "logits must be a GPU tensor");
+    TORCH_CHECK(logits.dim() == 2, "logits must be [rows, vocab], are ", logits.sizes());
+    TORCH_CHECK(io_type(logits.scalar_type()) >= 0, "logits must be float16, bfloat16 or float32");
+    refuse_gradient({&logits}, "sample");
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    TORCH_CHECK(rows >= 1 && rows <= 65535 && vocab >= 1 && vocab <= 1 << 20, "1 to 65535 rows of 1 to 2^20 logits, got ", logits.sizes());
+    const auto device = logits.device();
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
+    if (!rows_are(logits, 1, 1)) logits = logits.contiguous();
+    check_vector(uniform, "uniform", device, at::kFloat, rows);
+    if (temperature) check_vector(*temperature, "temperature", device, at::kFloat, rows);
+    if (top_k) check_vector(*top_k, "top_k", device, at::kInt, rows);
+    if (top_p) check_vector(*top_p, "top_p", device, at::kFloat, rows);
+    if (min_p) check_vector(*min_p, "min_p", device, at::kFloat, rows);
+    const at::Tensor ids(at::detail::empty_cuda({rows}, at::kLong, device, c10::nullopt)),
+        logprob(at::detail::empty_cuda({rows}, at::kFloat, device, c10::nullopt));
+    const size_t bytes = lutgemm_sampling_workspace((int)rows, (int)vocab);
+    const at::Tensor workspace = workspace_of(bytes, device);
+    auto floats = [](const at::Tensor *t) { return t ? (const float *)t->const_data_ptr() : nullptr; };
+    lutgemm_sampling c{};
+    c.logits = logits.const_data_ptr();
+    c.row_stride = rows > 1 ? logits.stride(0) : vocab;
+    c.logits_type = io_type(logits.scalar_type());
+    c.rows = (int)rows;
+    c.vocab = (int)vocab;
+    c.temperature = floats(temperature);
+    c.top_k = top_k ? (const int32_t *)top_k->const_data_ptr() : nullptr;
+    c.top_p = floats(top_p);
+    c.min_p = floats(min_p);
+    c.uniform = floats(&uniform);
+    c.ids = (int64_t *)ids.data_ptr();
+    c.logprob = (float *)logprob.data_ptr();
+    raise_on_error(lutgemm_sample_tokens(&c, bytes ? workspace.data_ptr() : nullptr, bytes,
+                                         c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream()), "sample");
+    return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(ids)).ptr(), py::reinterpret_steal<py::object>(THPVariable_Wrap(logprob)).ptr());
+    END_HANDLE_TH_ERRORS
+}
+
+// adapters_apply(x, ids, base, out, down, up, scale) -> out
+PyObject *adapters_apply_py(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 7, "adapters_apply takes 7 arguments, got ", n);
+    at::Tensor x = required_tensor(args[0], "x"), base = required_tensor(args[2], "base");
+    const at::Tensor &ids = required_tensor(args[1], "ids"), &down = required_tensor(args[4], "down"), &up = required_tensor(args[5], "up"),
+                     &scale = required_tensor(args[6], "scale");
+    const at::Tensor *given = optional_tensor(args[3], "out");
+    TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
+    const auto device = x.device();
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(device);
+    check_like(down, "down", device, at::kHalf);
+    check_like(up, "up", device, at::kHalf);
+    TORCH_CHECK(down.dim() == 3 && up.dim() == 3 && down.is_contiguous() && up.is_contiguous() && down.size(0) == up.size(0) && down.size(1) == up.size(2),
+                "down must be contiguous [adapters, rank, K] and up [adapters, N, rank], are ", down.sizes(), " and ", up.sizes());
+    const int64_t count = down.size(0), rank = down.size(1), K = down.size(2), N = up.size(1);
+    check_like(x, "x", device, at::kHalf);
+    check_like(base, "base", device, at::kHalf);
+    refuse_gradient({&x, &base, &down, &up, &scale}, "AdapterBank");
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == K, "expected last dimension ", K, ", got ", x.sizes());
+    TORCH_CHECK(x.numel() > 0, "the input is empty");
+    const int64_t M = x.numel() / K;
+    TORCH_CHECK(base.dim() == x.dim() && base.numel() == M * N && base.size(-1) == N && base.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                "base must have the shape of x with ", N, " columns, is ", base.sizes());
+    TORCH_CHECK(M <= 65535, "at most 65535 rows, got ", M);
+    check_vector(ids, "ids", device, at::kInt, M);
+    check_vector(scale, "scale", device, at::kFloat, count);
+    // (rows: two dimensions with any stride of the rows, or contiguous)
+    if (!(x.dim() <= 2 || x.is_contiguous()) || !rows_are(x, 8, 16)) x = x.clone(at::MemoryFormat::Contiguous);
+    if (!(base.dim() <= 2 || base.is_contiguous()) || !rows_are(base, 4, 8)) base = base.contiguous();
+    if ((uintptr_t)base.const_data_ptr() % 8 != 0) base = base.clone(at::MemoryFormat::Contiguous);
+    at::Tensor out;
+    if (given) {
+        check_like(*given, "out", device, at::kHalf);
+        TORCH_CHECK(given->sizes() == base.sizes() && (given->dim() <= 2 || given->is_contiguous()) && rows_are(*given, 4, 8),
+                    "out must have the shape of base, rows of contiguous values, 8-byte aligned");
+        out = *given;
+    } else {
+        out = at::Tensor(at::detail::empty_cuda(base.sizes(), at::kHalf, device, c10::nullopt));
+    }
+    auto row_stride = [&](const at::Tensor &t, int64_t columns) { return M == 1 ? columns : t.dim() == 2 ? t.stride(0) : columns; };
+    lutgemm_adapters p{};
+    p.x_f16 = x.const_data_ptr();
+    p.base_f16 = base.const_data_ptr();
+    p.out_f16 = out.data_ptr();
+    p.ids = (const int32_t *)ids.const_data_ptr();
+    p.down_f16 = down.const_data_ptr();
+    p.up_f16 = up.const_data_ptr();
+    p.scale = (const float *)scale.const_data_ptr();
+    p.x_stride = row_stride(x, K);
+    p.base_stride = row_stride(base, N);
+    p.out_stride = row_stride(out, N);
+    p.M = (int)M;
+    p.N = (int)N;
+    p.K = (int)K;
+    p.rank = (int)rank;
+    p.adapters = (int)count;
+    const size_t bytes = lutgemm_adapters_workspace(1, &p);
+    const at::Tensor workspace = workspace_of(bytes, device);
+    raise_on_error(lutgemm_adapters_f16(1, &p, bytes ? workspace.data_ptr() : nullptr, bytes,
+                                        c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream()), "AdapterBank");
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef served_defs[] = {
+    {"q4_attend", (PyCFunction)(void (*)(void))q4_attend_py, METH_FASTCALL,
+     "q4_attend(cache, q, k, v, cos, sin, start, counts, out, held, max_positions, /)\n--\n\nOne step over a cache held in 4 bits."},
+    {"sample_tokens", (PyCFunction)(void (*)(void))sample_tokens_py, METH_FASTCALL,
+     "sample_tokens(logits, uniform, temperature, top_k, top_p, min_p, /)\n--\n\nOne token per row of logits."},
+    {"adapters_apply", (PyCFunction)(void (*)(void))adapters_apply_py, METH_FASTCALL,
+     "adapters_apply(x, ids, base, out, down, up, scale, /)\n--\n\nbase + scale * up (down x), every row through its adapter."},
+};
+
 // Calibration copy for profiler byte counters (no reference counterpart).
 void copy_bytes(torch::Tensor dst, torch::Tensor src)
 {
@@ -473,5 +731,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("makeRandomWeight", &makeRandomWeight, "fill qW [K, NUM_BITS, N] with +-1 and bW [K/32, NUM_BITS, N] with their packing");
     m.def("parsing", &parsing, "host tensors -> flat device buffers {bWeight, q_bias, alpha}");
     m.add_object("linear_forward", py::reinterpret_steal<py::object>(PyCFunction_New(&linear_forward_def, nullptr)));
+    for (PyMethodDef &def : served_defs) m.add_object(def.ml_name, py::reinterpret_steal<py::object>(PyCFunction_New(&def, nullptr)));
     m.def("copy_bytes", &copy_bytes, "calibration copy kernel");
 }

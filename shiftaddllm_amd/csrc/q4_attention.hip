@@ -1,0 +1,648 @@
+// Attention over a cache of keys and values held in 4 bits, gfx950: appending of new tokens, attention of one or many query
+// rows, joining of what workgroups found over different positions.  The layout and the rules of rounding are in lutgemm_gfx950.h.
+//
+// Mathematics.  For a (sequence, kv head) pair the query rows are (token, query head) pairs, row = token * rep + member.
+// Scores are formed transposed, S^T = K Q^T: the matrix instruction's A operand is 16 positions of keys, B 16 query rows, so
+// that a lane ends up with one query row (lane % 16) and four positions of either half of a block of 32.  Those eight weights
+// are, as they are, the B operand of O^T = V^T P^T when the values of a block are stored with the positions in that order,
+// eight to a word: no value crosses lanes between the two products, and what a row is rescaled by is a lane's own scalar.
+// A held value is one fp16 number, fp16(minimum + scale * code); it is formed in registers (a shift, and-or, an exact
+// subtraction and an fma for two values) and multiplied exactly, sums in fp32.
+// Softmax keeps a reference per row, not the exact maximum: it is raised only when a score exceeds it by 2^8, so that most
+// blocks need no exchange between lanes.  Weights, at most 2^8, are rounded to fp16 for the matrix product (half a step, 2^-11 relative,
+// where they are 2^-14 or more; the error of a sum over many positions averages out); their sum is formed in fp32 from the unrounded ones.
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "lutgemm_gfx950.h"
+#include "lutgemm_common.h"
+#include "lutgemm_internal.h"
+
+namespace {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kBlock = 32;              // positions of a block of the cache
+constexpr float kLargest = 60000.0f;    // of a held number
+constexpr float kSlack = 8.0f;          // by which (in powers of two) a score may exceed its row's reference
+
+struct Args {
+    uint8_t *cache;
+    const _Float16 *q, *k, *v, *cos_t, *sin_t;
+    const int64_t *start;
+    const int32_t *counts;
+    _Float16 *out, *k_held, *v_held;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+    int tokens, heads, kv_heads, rep, max_positions, blocks;   // blocks: of a (sequence, kv head) pair in the cache
+    int pairs, units, tiles, splits;                           // units: tiles of a wave's rows; tiles: of a workgroup's
+    float *partial;                                            // [split][pair][unit][rows][head_dim], then ...
+    float2 *stats;                                             // ... (reference, sum) [split][pair][unit][rows]
+};
+
+// A sequence's new tokens: the first one's position and how many there are (0: all are passed over).
+__device__ __forceinline__ int live_tokens(const Args &a, int b, int &start)
+{
+    const int64_t s = a.start[b];
+    int n = a.counts ? a.counts[b] : a.tokens;
+    n = min(max(n, 0), a.tokens);
+    start = 0;
+    if (s < 0 || s >= a.max_positions) return 0;
+    start = (int)s;
+    return min(n, a.max_positions - start);
+}
+
+// Eight numbers at dimensions d .. d + 7 of a head, rotated by the angles of a position and rounded to fp16.
+__device__ __forceinline__ f16x8 rotated(const _Float16 *head, const _Float16 *cos_row, const _Float16 *sin_row, int d, int hd)
+{
+    const int half = hd / 2;
+    const f16x8 x = *(const f16x8 *)(head + d), y = *(const f16x8 *)(head + (d < half ? d + half : d - half));
+    const f16x8 c = *(const f16x8 *)(cos_row + d), s = *(const f16x8 *)(sin_row + d);
+    const float sign = d < half ? -1.0f : 1.0f;
+    f16x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // (products of fp16 numbers are exact in fp32; the sum is rounded to fp32 and then to fp16, as framework operations round it:
+        // without the empty statement one instruction would round once)
+        float sum = (float)x[i] * (float)c[i] + sign * (float)y[i] * (float)s[i];
+        asm volatile("" : "+v"(sum));
+        r[i] = (_Float16)sum;
+    }
+    return r;
+}
+
+// What a group of 32 numbers is held as, by the four neighbouring lanes that have eight each.
+struct Held {
+    _Float16 scale, low;
+    uint32_t codes;   // of this lane's numbers, 4 bits each, number i at bit 4 i
+    f16x8 value;
+};
+
+__device__ __forceinline__ Held quantise(f16x8 x)
+{
+    Held h;
+    float f[8], low = kLargest, high = -kLargest;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = (float)x[i];
+        f[i] = v != v ? 0.0f : fminf(fmaxf(v, -kLargest), kLargest);
+        low = fminf(low, f[i]);
+        high = fmaxf(high, f[i]);
+    }
+#pragma unroll
+    for (int m = 1; m < 4; m *= 2) {
+        low = fminf(low, __shfl_xor(low, m));
+        high = fmaxf(high, __shfl_xor(high, m));
+    }
+    h.low = (_Float16)low;   // (exact: one of the numbers, or +-60000)
+    h.scale = (_Float16)(float)(((double)high - (double)low) / 15.0);
+    const double s = (double)(float)h.scale;
+    const float inverse = (float)h.scale > 0.0f ? 1.0f / (float)h.scale : 0.0f;
+    h.codes = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // The nearest code, exactly: the quotient in fp32 is off by far less than one, what is left over is exact in 64 bits.
+        int c = (int)fminf(rintf((f[i] - low) * inverse), 15.0f);
+        const double rest = ((double)f[i] - (double)low) - c * s;
+        if (2.0 * rest > s || (2.0 * rest == s && (c & 1))) ++c;
+        else if (-2.0 * rest > s || (-2.0 * rest == s && (c & 1))) --c;
+        c = s > 0.0 ? min(max(c, 0), 15) : 0;
+        h.codes |= (uint32_t)c << (4 * i);
+        h.value[i] = __builtin_fmaf16((_Float16)(float)c, h.scale, h.low);
+    }
+    return h;
+}
+
+// The word in which eight codes are kept, from them in order: even ones in the low half.
+__device__ __forceinline__ uint32_t word_of(uint32_t codes)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= ((codes >> (4 * e)) & 15u) << (4 * (e / 2) + 16 * (e & 1));
+    return w;
+}
+
+// One workgroup per block of the cache that new tokens of a (sequence, kv head) pair fall into: it alone writes the block, so that
+// words that hold other positions too can be read, changed and written.  Lanes 4 i .. 4 i + 3 take a group of 32 numbers.
+template <int G>
+__global__ void __launch_bounds__(kThreads) append_kernel(const Args a)
+{
+    constexpr int HD = 32 * G;
+    __shared__ uint8_t code[kBlock][HD + 4];   // of the values, by position
+    const int tid = threadIdx.x;
+    const int pair = blockIdx.x % a.pairs, part = blockIdx.x / a.pairs;
+    const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
+    int start;
+    const int n = live_tokens(a, b, start);
+    const size_t held_row = (size_t)a.kv_heads * HD;
+    if (a.k_held || a.v_held) {   // rows of tokens that are passed over
+        for (int u = tid; u < kBlock * (HD / 8); u += kThreads) {
+            const int token = part * kBlock + u / (HD / 8);
+            if (token < n || token >= a.tokens) continue;
+            const size_t at = ((size_t)b * a.tokens + token) * held_row + (size_t)kvh * HD + u % (HD / 8) * 8;
+            if (a.k_held) *(u32x4 *)(a.k_held + at) = (u32x4){0, 0, 0, 0};
+            if (a.v_held) *(u32x4 *)(a.v_held + at) = (u32x4){0, 0, 0, 0};
+        }
+    }
+    const int block = start / kBlock + part;
+    const int first = block * kBlock - start;   // token of the block's first position
+    if (n == 0 || first >= n) return;
+    uint8_t *base = a.cache + ((size_t)pair * a.blocks + block) * (size_t)(1280 * G);
+    uint32_t *k_codes = (uint32_t *)base;
+    uint32_t *k_scales = (uint32_t *)(base + 512 * G);
+    uint32_t *v_codes = (uint32_t *)(base + 640 * G);
+    _Float16 *v_scales = (_Float16 *)(base + 1152 * G);
+
+    for (int u = tid; u < kBlock * G * 4; u += kThreads) {
+        const int quad = u % 4, t = u / 4 % G, p = u / (4 * G);
+        const int token = first + p, d = 32 * t + 8 * quad;
+        const bool live = token >= 0 && token < n;
+        const int row = live ? token : 0;
+        const _Float16 *kh = a.k + b * a.k_stride[0] + row * a.k_stride[1] + (size_t)kvh * HD;
+        const _Float16 *vh = a.v + b * a.v_stride[0] + row * a.v_stride[1] + (size_t)kvh * HD;
+        const size_t angle = (size_t)(start + row) * HD;
+        const Held hk = quantise(rotated(kh, a.cos_t + angle, a.sin_t + angle, d, HD));
+        const Held hv = quantise(*(const f16x8 *)(vh + d));
+        if (!live) continue;
+        k_codes[(p * 4 + quad) * G + t] = word_of(hk.codes);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[p][d + i] = (uint8_t)((hv.codes >> (4 * i)) & 15u);
+        if (quad == 0) {
+            const f16x2 pair_of = {hk.scale, hk.low};
+            k_scales[p * G + t] = __builtin_bit_cast(uint32_t, pair_of);
+            const int slot = p % 16 / 4 * 8 + p / 16 * 4 + p % 4;
+            v_scales[(2 * t) * kBlock + slot] = hv.scale;
+            v_scales[(2 * t + 1) * kBlock + slot] = hv.low;
+        }
+        const size_t at = ((size_t)b * a.tokens + token) * held_row + (size_t)kvh * HD + d;
+        if (a.k_held) *(f16x8 *)(a.k_held + at) = hk.value;
+        if (a.v_held) *(f16x8 *)(a.v_held + at) = hv.value;
+    }
+    __syncthreads();
+    for (int u = tid; u < 128 * G; u += kThreads) {
+        const int t = u % (2 * G), column = u / (2 * G) % 16, quad = u / (32 * G);
+        uint32_t fresh = 0, mask = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int p = 4 * quad + e % 4 + 16 * (e / 4), shift = 4 * (e / 2) + 16 * (e & 1);
+            if (first + p < 0 || first + p >= n) continue;
+            fresh |= (uint32_t)code[p][16 * t + column] << shift;
+            mask |= 15u << shift;
+        }
+        if (mask) v_codes[u] = mask == ~0u ? fresh : (v_codes[u] & ~mask) | fresh;
+    }
+}
+
+// Two held values from bits 4 I .. of either half of a word (I = 0, 1): the code, put into the low bits of the significand of 1024 (64), is
+// 1024 + code (64 + code) as it stands.
+template <int I>
+__device__ __forceinline__ f16x2 code_pair(uint32_t w)
+{
+    const uint32_t bits = I == 0 ? (w & 0x000f000fu) | 0x64006400u : (w & 0x00f000f0u) | 0x54005400u;
+    const _Float16 off = I == 0 ? (_Float16)1024.0f : (_Float16)64.0f;
+    return __builtin_bit_cast(f16x2, bits) - (f16x2){off, off};
+}
+
+__device__ __forceinline__ f16x8 codes_of(uint32_t w)
+{
+    const uint32_t u = w >> 8;
+    const f16x2 p0 = code_pair<0>(w), p1 = code_pair<1>(w), p2 = code_pair<0>(u), p3 = code_pair<1>(u);
+    return (f16x8){p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&to)[N], const void *from)
+{
+    __builtin_memcpy(to, from, 4 * N);
+}
+
+// Blocks of a tile that new rows up to position `last` attend to, and how they are shared by the workgroups of its positions.
+__device__ __forceinline__ int blocks_per_split(const Args &a, int blocks, int least)
+{
+    return max((blocks + a.splits - 1) / a.splits, least);
+}
+
+// A wave takes 16 RT query rows of a (sequence, kv head) pair.  APART: the waves of a workgroup take different rows and all of
+// the workgroup's blocks (long prompts); otherwise they take the same rows, and the blocks in turn.
+template <int G, int RT, bool APART>
+__global__ void __launch_bounds__(kThreads) attention_kernel(const Args a)
+{
+    constexpr int HD = 32 * G, ROWS = 16 * RT;
+    constexpr int kTilesAtOnce = RT == 1 ? 8 : 4;   // of 16 dimensions, joined at a time
+    constexpr int kPadded = 16 * kTilesAtOnce + 4;
+    __shared__ float joined[APART ? 1 : kWaves][APART ? 1 : ROWS][APART ? 1 : kPadded];
+    __shared__ float2 wave_stats[kWaves][ROWS];
+
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int column = lane & 15, quad = lane >> 4;
+    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int split = rest % a.splits, tile = a.tiles - 1 - rest / a.splits;   // (the longest rows of a prompt first)
+    const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
+    int start;
+    const int n = live_tokens(a, b, start);
+    const int unit = APART ? tile * kWaves + wave : tile;
+    const int row0 = unit * ROWS, all_rows = a.tokens * a.rep, live_rows = n * a.rep;
+
+    // the blocks of this workgroup
+    const int tile_rows = APART ? kWaves * ROWS : ROWS;
+    const int tile_last = min((tile + 1) * tile_rows, live_rows) - 1;          // its last row that is no padding
+    const int tile_blocks = tile_last >= tile * tile_rows ? (start + tile_last / a.rep) / kBlock + 1 : 0;
+    const int per = blocks_per_split(a, tile_blocks, APART ? 4 : kWaves);
+    const int begin = split * per;
+    int end = min(begin + per, tile_blocks);
+    const int last = min(row0 + ROWS, live_rows) - 1;                          // of this wave
+    const int limit_high = last >= row0 ? start + last / a.rep : -1, limit_low = start + row0 / a.rep;
+    if (APART) end = min(end, (limit_high + kBlock) / kBlock);
+    if (!APART && a.splits > 1 && begin >= end) return;                        // (nobody reads its part)
+
+    f16x8 q[RT][G];
+    int limit[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row0 + 16 * rt + column, max(live_rows, 1) - 1), token = row / a.rep;
+        limit[rt] = start + token;
+        const _Float16 *head = a.q + b * a.q_stride[0] + token * a.q_stride[1] + (size_t)(kvh * a.rep + row % a.rep) * HD;
+        const size_t angle = (size_t)(start + token) * HD;
+#pragma unroll
+        for (int t = 0; t < G; ++t) q[rt][t] = rotated(head, a.cos_t + angle, a.sin_t + angle, 32 * t + 8 * quad, HD);
+    }
+
+    f32x4 acc[RT][2 * G];
+    float reference[RT], sum[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        reference[rt] = -1e30f;
+        sum[rt] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t) acc[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const float to_log2 = 1.4426950408889634f / sqrtf((float)HD);
+    const uint8_t *cache = a.cache + (size_t)pair * a.blocks * (size_t)(1280 * G);
+
+    uint32_t k_codes[2][G], k_scales[2][G], v_codes[2 * G], v_scales[2 * G][4];
+    auto fetch_keys = [&](int block) {
+        const uint8_t *base = cache + (size_t)block * (1280 * G);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            load_words(k_codes[h], base + ((16 * h + column) * 4 + quad) * (4 * G));
+            load_words(k_scales[h], base + 512 * G + (16 * h + column) * (4 * G));
+        }
+    };
+    auto fetch_values = [&](int block) {
+        const uint8_t *base = cache + (size_t)block * (1280 * G) + 640 * G;
+        load_words(v_codes, base + (quad * 16 + column) * (8 * G));
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t) load_words(v_scales[t], base + 512 * G + t * 64 + quad * 16);
+    };
+    const int step = APART ? 1 : kWaves;
+    int block = begin + (APART ? 0 : wave);
+    if (block < end) {
+        fetch_keys(block);
+        fetch_values(block);
+    }
+    for (; block < end; block += step) {
+        const int next = block + step < end ? block + step : block;
+        f32x4 score[RT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) score[rt][h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int t = 0; t < G; ++t) {
+                const f16x2 sm = __builtin_bit_cast(f16x2, k_scales[h][t]);
+                const f16x8 key = __builtin_elementwise_fma(codes_of(k_codes[h][t]), (f16x8)(sm.x), (f16x8)(sm.y));
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) score[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[rt][t], score[rt][h], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_keys(next);
+        __builtin_amdgcn_sched_barrier(0);
+        const int j0 = block * kBlock;
+        const bool edge = j0 + kBlock - 1 > limit_low;
+        f16x8 weight[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float s[8], most = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = score[rt][e / 4][e % 4] * to_log2;
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] = j0 + 16 * (e / 4) + 4 * quad + e % 4 <= limit[rt] ? s[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, s[e]);
+            if (__any(most > reference[rt] + kSlack)) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const float raised = fmaxf(reference[rt], most), keep = __builtin_amdgcn_exp2f(reference[rt] - raised);
+                reference[rt] = raised;
+                sum[rt] *= keep;
+#pragma unroll
+                for (int t = 0; t < 2 * G; ++t) acc[rt][t] *= keep;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = __builtin_amdgcn_exp2f(s[e] - reference[rt]);
+                sum[rt] += p;
+                weight[rt][e] = (_Float16)p;
+            }
+        }
+        if (j0 + kBlock - 1 > limit_high) {   // positions that no row attends to: whatever is there, times zero
+            uint32_t mask[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int p = j0 + 16 * (i / 2) + 4 * quad + 2 * (i % 2);
+                mask[i] = (p <= limit_high ? 0xffffu : 0u) | (p + 1 <= limit_high ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * G; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v_scales[t][i] &= mask[i];
+        }
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t) {
+            const f16x8 scale = __builtin_bit_cast(f16x8, (u32x4){v_scales[t & ~1][0], v_scales[t & ~1][1], v_scales[t & ~1][2], v_scales[t & ~1][3]});
+            const f16x8 low = __builtin_bit_cast(f16x8, (u32x4){v_scales[t | 1][0], v_scales[t | 1][1], v_scales[t | 1][2], v_scales[t | 1][3]});
+            const f16x8 value = __builtin_elementwise_fma(codes_of(v_codes[t]), scale, low);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], acc[rt][t], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_values(next);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        sum[rt] += __shfl_xor(sum[rt], 16);
+        sum[rt] += __shfl_xor(sum[rt], 32);
+    }
+
+    // ---- the rows' results: out, or this split's part -----------------------------------------------------------------------
+    // Four numbers of a row at dimension d: `value` / total, or value with the row's reference and total beside it.
+    auto store = [&](int row, int d, f32x4 value, float reference_, float total) {
+        if (row >= all_rows) return;
+        if (a.splits > 1) {
+            const size_t at = (((size_t)split * a.pairs + pair) * a.units + unit) * ROWS + (row - row0);
+            *(f32x4 *)(a.partial + at * HD + d) = value;
+            if (d == 0) a.stats[at] = make_float2(reference_, total);
+            return;
+        }
+        const int token = row / a.rep;
+        const float inverse = row < live_rows ? 1.0f / total : 0.0f;
+        if (row >= live_rows) value = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+        const f16x4 o = {(_Float16)(value[0] * inverse), (_Float16)(value[1] * inverse), (_Float16)(value[2] * inverse), (_Float16)(value[3] * inverse)};
+        *(f16x4 *)(a.out + (((size_t)b * a.tokens + token) * a.heads + kvh * a.rep + row % a.rep) * HD + d) = o;
+    };
+    if constexpr (APART) {
+        if (unit >= a.units) return;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int t = 0; t < 2 * G; ++t) store(row0 + 16 * rt + column, 16 * t + 4 * quad, acc[rt][t], reference[rt], sum[rt]);
+    } else {
+        if (quad == 0)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) wave_stats[wave][16 * rt + column] = make_float2(reference[rt], sum[rt]);
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float most = -1e30f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) most = fmaxf(most, wave_stats[w][16 * rt + column].x);
+            const float keep = __builtin_amdgcn_exp2f(reference[rt] - most);
+#pragma unroll
+            for (int t = 0; t < 2 * G; ++t) acc[rt][t] *= keep;
+        }
+#pragma unroll
+        for (int t0 = 0; t0 < 2 * G; t0 += kTilesAtOnce) {
+            if (t0 > 0) __syncthreads();
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int t = t0; t < t0 + kTilesAtOnce && t < 2 * G; ++t)
+                    *(f32x4 *)&joined[wave][16 * rt + column][16 * (t - t0) + 4 * quad] = acc[rt][t];
+            __syncthreads();
+            const int fours = 4 * min(kTilesAtOnce, 2 * G - t0);
+            for (int u = tid; u < ROWS * fours; u += kThreads) {
+                const int row = u / fours, d = u % fours * 4;
+                f32x4 value = *(const f32x4 *)&joined[0][row][d];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) value += *(const f32x4 *)&joined[w][row][d];
+                float most = -1e30f, total = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) most = fmaxf(most, wave_stats[w][row].x);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) total += wave_stats[w][row].y * __builtin_amdgcn_exp2f(wave_stats[w][row].x - most);
+                store(row0 + row, 16 * t0 + d, value, most, total);
+            }
+        }
+    }
+}
+
+// Joins the parts of a row: sum over splits of 2^(reference - largest reference) * part, in the order of the splits.
+// One thread per four dimensions of a row.
+template <int G>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Args a, int rows_per_unit, int units_per_tile)
+{
+    constexpr int HD = 32 * G;
+    const int all_rows = a.tokens * a.rep;
+    const long u = (long)blockIdx.x * kThreads + threadIdx.x;
+    const int d = (int)(u % (HD / 4)) * 4;
+    const long at_row = u / (HD / 4);
+    const int pair = (int)(at_row / all_rows), row = (int)(at_row % all_rows);
+    if (pair >= a.pairs) return;
+    const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
+    int start;
+    const int n = live_tokens(a, b, start), live_rows = n * a.rep;
+    const int unit = row / rows_per_unit, tile = unit / units_per_tile, tile_rows = units_per_tile * rows_per_unit;
+    f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+    float total = 1.0f;
+    if (row < live_rows) {
+        const int tile_last = min((tile + 1) * tile_rows, live_rows) - 1;
+        const int tile_blocks = (start + tile_last / a.rep) / kBlock + 1;
+        const int per = blocks_per_split(a, tile_blocks, units_per_tile > 1 ? 4 : kWaves);
+        const int parts = (tile_blocks + per - 1) / per;
+        const size_t stride = (size_t)a.pairs * a.units * rows_per_unit;
+        const size_t at = ((size_t)pair * a.units + unit) * rows_per_unit + row % rows_per_unit;
+        float most = -1e30f;
+        for (int s = 0; s < parts; ++s) most = fmaxf(most, a.stats[s * stride + at].x);
+        total = 0.0f;
+        for (int s = 0; s < parts; ++s) {
+            const float2 st = a.stats[s * stride + at];
+            const float keep = __builtin_amdgcn_exp2f(st.x - most);
+            total += st.y * keep;
+            value += *(const f32x4 *)(a.partial + (s * stride + at) * HD + d) * keep;
+        }
+    }
+    const float inverse = 1.0f / total;
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    const f16x4 o = {(_Float16)(value[0] * inverse), (_Float16)(value[1] * inverse), (_Float16)(value[2] * inverse), (_Float16)(value[3] * inverse)};
+    *(f16x4 *)(a.out + (((size_t)b * a.tokens + row / a.rep) * a.heads + kvh * a.rep + row % a.rep) * HD + d) = o;
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+
+int launch_status()
+{
+    hipError_t e = hipGetLastError();
+    return e == hipSuccess ? LUTGEMM_OK : lutgemm_internal_hip_fail((int)e);
+}
+
+bool cache_sizes_fit(int batch, int kv_heads, int max_positions, int head_dim)
+{
+    return batch >= 1 && batch <= 65535 && kv_heads >= 1 && kv_heads <= 4096 && max_positions >= 1 && max_positions <= 1 << 20 &&
+           head_dim >= 32 && head_dim <= 256 && head_dim % 32 == 0;
+}
+
+struct Sizes {
+    int units, tiles;
+    size_t partial_floats;   // of the whole call
+    size_t workspace;
+};
+
+int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_positions, lutgemm_q4_attention_plan *p, Sizes *s)
+{
+    if (!cache_sizes_fit(batch, kv_heads, max_positions, head_dim) || tokens < 1 || tokens > 65536) return LUTGEMM_EINVAL;
+    if (heads < kv_heads || heads > 4096 || heads % kv_heads != 0) return LUTGEMM_EINVAL;
+    const long rows = (long)tokens * (heads / kv_heads), pairs = (long)batch * kv_heads;
+    const int blocks = (max_positions + kBlock - 1) / kBlock;
+    p->fused = 0;
+    p->threads = kThreads;
+    p->rows_per_wave = rows > 16 ? 32 : 16;
+    p->rows_apart = rows >= 4 * 32;
+    s->units = (int)((rows + p->rows_per_wave - 1) / p->rows_per_wave);
+    s->tiles = p->rows_apart ? (s->units + kWaves - 1) / kWaves : s->units;
+    const long alone = pairs * s->tiles;
+    long splits = 1;
+    if (alone < 1024) splits = (1024 + alone - 1) / alone;
+    const long most = blocks / (p->rows_apart ? 32 : 32);   // each split has some blocks to itself
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+    p->splits = (int)splits;
+    p->row_tiles = s->tiles;
+    p->launches = splits > 1 ? 3 : 2;
+    if (alone * splits > 0x7fffffffl || pairs * ((tokens + kBlock - 1) / kBlock + 1) > 0x7fffffffl) return LUTGEMM_EINVAL;
+    p->workgroups = (int)(alone * splits);
+    const size_t part_rows = (size_t)splits * pairs * s->units * p->rows_per_wave;
+    s->partial_floats = splits > 1 ? part_rows * head_dim : 0;
+    s->workspace = splits > 1 ? part_rows * (head_dim * 4 + 8) : 0;
+    if ((size_t)pairs * tokens * (heads / kv_heads) * (head_dim / 4) / kThreads > 0x7ffffff0u) return LUTGEMM_EINVAL;
+    return LUTGEMM_OK;
+}
+
+bool strides_fit(const int64_t (&s)[2], const void *p)
+{
+    return aligned16(p) && s[0] % 8 == 0 && s[1] % 8 == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t lutgemm_q4_cache_bytes(int batch, int kv_heads, int max_positions, int head_dim)
+{
+    if (!cache_sizes_fit(batch, kv_heads, max_positions, head_dim)) return 0;
+    return (size_t)batch * kv_heads * ((max_positions + kBlock - 1) / kBlock) * (size_t)(40 * head_dim);
+}
+
+size_t lutgemm_q4_attention_workspace(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_positions)
+{
+    lutgemm_q4_attention_plan plan;
+    Sizes sizes;
+    if (plan_call(batch, tokens, heads, kv_heads, head_dim, max_positions, &plan, &sizes) != LUTGEMM_OK) return 0;
+    return sizes.workspace;
+}
+
+int lutgemm_describe_q4_attention_plan(int batch, int tokens, int heads, int kv_heads, int head_dim, int max_positions,
+                                       lutgemm_q4_attention_plan *plan)
+{
+    if (!plan) return LUTGEMM_EINVAL;
+    Sizes sizes;
+    return plan_call(batch, tokens, heads, kv_heads, head_dim, max_positions, plan, &sizes);
+}
+
+int lutgemm_q4_attention_f16(const lutgemm_q4_attention *c, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!c || !c->cache || !c->q || !c->k || !c->v || !c->cos_table || !c->sin_table || !c->start || !c->out) return LUTGEMM_EINVAL;
+    lutgemm_q4_attention_plan plan;
+    Sizes sizes;
+    const int rc = plan_call(c->batch, c->tokens, c->heads, c->kv_heads, c->head_dim, c->max_positions, &plan, &sizes);
+    if (rc != LUTGEMM_OK) return rc;
+    for (int i = 0; i < 2; ++i)
+        if (c->q_stride[i] < 0 || c->k_stride[i] < 0 || c->v_stride[i] < 0) return LUTGEMM_EINVAL;
+    if (sizes.workspace > 0 && (!workspace || workspace_bytes < sizes.workspace)) return LUTGEMM_EINVAL;
+    if (!aligned16(c->cache) || !aligned16(c->cos_table) || !aligned16(c->sin_table) || !aligned16(c->out) || !aligned16(c->k_held) ||
+        !aligned16(c->v_held) || ((uintptr_t)c->start & 7u) || ((uintptr_t)c->counts & 3u) || (sizes.workspace > 0 && !aligned16(workspace)) ||
+        !strides_fit(c->q_stride, c->q) || !strides_fit(c->k_stride, c->k) || !strides_fit(c->v_stride, c->v))
+        return LUTGEMM_EALIGN;
+    Args a{};
+    a.cache = (uint8_t *)c->cache;
+    a.q = (const _Float16 *)c->q;
+    a.k = (const _Float16 *)c->k;
+    a.v = (const _Float16 *)c->v;
+    a.cos_t = (const _Float16 *)c->cos_table;
+    a.sin_t = (const _Float16 *)c->sin_table;
+    a.start = c->start;
+    a.counts = c->counts;
+    a.out = (_Float16 *)c->out;
+    a.k_held = (_Float16 *)c->k_held;
+    a.v_held = (_Float16 *)c->v_held;
+    for (int i = 0; i < 2; ++i) {
+        a.q_stride[i] = c->q_stride[i];
+        a.k_stride[i] = c->k_stride[i];
+        a.v_stride[i] = c->v_stride[i];
+    }
+    a.tokens = c->tokens;
+    a.heads = c->heads;
+    a.kv_heads = c->kv_heads;
+    a.rep = c->heads / c->kv_heads;
+    a.max_positions = c->max_positions;
+    a.blocks = (c->max_positions + kBlock - 1) / kBlock;
+    a.pairs = c->batch * c->kv_heads;
+    a.units = sizes.units;
+    a.tiles = sizes.tiles;
+    a.splits = plan.splits;
+    a.partial = (float *)workspace;
+    a.stats = (float2 *)((float *)workspace + sizes.partial_floats);
+    const hipStream_t hs = (hipStream_t)stream;
+
+    auto run = [&](auto g_c) -> int {
+        constexpr int G = decltype(g_c)::value;
+        const long parts = (a.tokens + kBlock - 1) / kBlock + 1;
+        hipLaunchKernelGGL(append_kernel<G>, dim3((unsigned)(parts * a.pairs)), dim3(kThreads), 0, hs, a);
+        int status = launch_status();
+        if (status != LUTGEMM_OK) return status;
+        const dim3 grid((unsigned)plan.workgroups);
+        if (plan.rows_apart) hipLaunchKernelGGL((attention_kernel<G, 2, true>), grid, dim3(kThreads), 0, hs, a);
+        else if (plan.rows_per_wave == 32) hipLaunchKernelGGL((attention_kernel<G, 2, false>), grid, dim3(kThreads), 0, hs, a);
+        else hipLaunchKernelGGL((attention_kernel<G, 1, false>), grid, dim3(kThreads), 0, hs, a);
+        status = launch_status();
+        if (status != LUTGEMM_OK || a.splits == 1) return status;
+        const size_t threads = (size_t)a.pairs * a.tokens * a.rep * (8 * G);
+        hipLaunchKernelGGL(join_kernel<G>, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, hs, a, plan.rows_per_wave,
+                           plan.rows_apart ? kWaves : 1);
+        return launch_status();
+    };
+    switch (c->head_dim / 32) {
+    case 1: return run(std::integral_constant<int, 1>());
+    case 2: return run(std::integral_constant<int, 2>());
+    case 3: return run(std::integral_constant<int, 3>());
+    case 4: return run(std::integral_constant<int, 4>());
+    case 5: return run(std::integral_constant<int, 5>());
+    case 6: return run(std::integral_constant<int, 6>());
+    case 7: return run(std::integral_constant<int, 7>());
+    default: return run(std::integral_constant<int, 8>());
+    }
+}
+
+}  // extern "C"

@@ -57,6 +57,14 @@ C_ABI_SYMBOLS = (
     "lutgemm_decode_silu_mul_f16",
     "lutgemm_gemv_rowwise_f16_gated",
     "lutgemm_describe_group_plan",
+    "lutgemm_q4_cache_bytes",
+    "lutgemm_q4_attention_workspace",
+    "lutgemm_q4_attention_f16",
+    "lutgemm_describe_q4_attention_plan",
+    "lutgemm_sampling_workspace",
+    "lutgemm_sample_tokens",
+    "lutgemm_adapters_workspace",
+    "lutgemm_adapters_f16",
 )
 
 
@@ -129,6 +137,34 @@ class GroupPlan(ctypes.Structure):
 class AttentionPlan(ctypes.Structure):
     """struct lutgemm_attention_plan of include/lutgemm_gfx950.h."""
     _fields_ = [(n, ctypes.c_int) for n in ("general", "workgroups", "threads", "placed", "once")]
+
+
+class Q4Attention(ctypes.Structure):
+    """struct lutgemm_q4_attention of include/lutgemm_gfx950.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("cache", "q", "k", "v", "cos_table", "sin_table", "start", "counts", "out",
+                                               "k_held", "v_held")] + \
+               [(n, ctypes.c_int64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [(n, ctypes.c_int) for n in ("batch", "tokens", "heads", "kv_heads", "head_dim", "max_positions")]
+
+
+class Q4AttentionPlan(ctypes.Structure):
+    """struct lutgemm_q4_attention_plan of include/lutgemm_gfx950.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("launches", "fused", "rows_per_wave", "row_tiles", "rows_apart", "splits",
+                                            "workgroups", "threads")]
+
+
+class Sampling(ctypes.Structure):
+    """struct lutgemm_sampling of include/lutgemm_gfx950.h."""
+    _fields_ = [("logits", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("logits_type", ctypes.c_int),
+                ("rows", ctypes.c_int), ("vocab", ctypes.c_int)] + \
+               [(n, ctypes.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p", "uniform", "ids", "logprob")]
+
+
+class Adapters(ctypes.Structure):
+    """struct lutgemm_adapters of include/lutgemm_gfx950.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x_f16", "base_f16", "out_f16", "ids", "down_f16", "up_f16", "scale")] + \
+               [(n, ctypes.c_int64) for n in ("x_stride", "base_stride", "out_stride")] + \
+               [(n, ctypes.c_int) for n in ("M", "N", "K", "rank", "adapters")]
 
 
 class NativeLibraryMissing(ImportError):
@@ -231,6 +267,22 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.lutgemm_gemv_rowwise_f16_gated.restype = ci
     lib.lutgemm_describe_group_plan.argtypes = [ci, ctypes.POINTER(FusedProblem), ctypes.POINTER(GroupPlan)]
     lib.lutgemm_describe_group_plan.restype = ci
+    lib.lutgemm_q4_cache_bytes.argtypes = [ci] * 4
+    lib.lutgemm_q4_cache_bytes.restype = sz
+    lib.lutgemm_q4_attention_workspace.argtypes = [ci] * 6
+    lib.lutgemm_q4_attention_workspace.restype = sz
+    lib.lutgemm_q4_attention_f16.argtypes = [ctypes.POINTER(Q4Attention), vp, sz, vp]
+    lib.lutgemm_q4_attention_f16.restype = ci
+    lib.lutgemm_describe_q4_attention_plan.argtypes = [ci] * 6 + [ctypes.POINTER(Q4AttentionPlan)]
+    lib.lutgemm_describe_q4_attention_plan.restype = ci
+    lib.lutgemm_sampling_workspace.argtypes = [ci, ci]
+    lib.lutgemm_sampling_workspace.restype = sz
+    lib.lutgemm_sample_tokens.argtypes = [ctypes.POINTER(Sampling), vp, sz, vp]
+    lib.lutgemm_sample_tokens.restype = ci
+    lib.lutgemm_adapters_workspace.argtypes = [ci, ctypes.POINTER(Adapters)]
+    lib.lutgemm_adapters_workspace.restype = sz
+    lib.lutgemm_adapters_f16.argtypes = [ci, ctypes.POINTER(Adapters), vp, sz, vp]
+    lib.lutgemm_adapters_f16.restype = ci
     lib.lutgemm_set_timestamp_buffer.argtypes = [vp, sz]
     lib.lutgemm_set_timestamp_buffer.restype = ci
     return lib
