@@ -3,12 +3,15 @@
 // Mathematics.  The order is larger logits first, equal ones by index, and every filter keeps a first part of it: the row's
 // tokens are never sorted, only the element is looked for at which a running count or a running sum of weights reaches a target.  The
 // weights, exp((l - m) / temperature) in 64 bits, are held as whole numbers of 2^-bits, so that sums do not depend on the order in
-// which threads add; as many bits as leave room for the sum of a vocabulary, 43 (2^20 tokens) to 52.  A histogram of counts and sums over 4096 equal steps of the logit
+// which threads add; as many bits as leave room for the sum of a vocabulary, 43 (2^20 tokens) to 51.  A histogram of counts and sums over 4096 equal steps of the logit
 // below the largest, as far as weights reach, says in which step a target is reached; the few tokens of that step are then looked
 // at one by one.  Where they are many (equal logits, an endless temperature) digits of the logit's bits are followed instead.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "lutgemm_gfx950.h"
 #include "lutgemm_common.h"
@@ -20,37 +23,48 @@ constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kSteps = 4096;          // of the histogram
 constexpr int kPerThread = kSteps / kThreads;
-constexpr int kList = 1024;           // tokens of a step that are looked at one by one, at most
+constexpr int kNear = 4096;           // tokens near the largest that are kept by themselves, at most
+constexpr int kMembers = 1024;        // tokens of a step that are looked at one by one, at most
+constexpr int kParts = 8;            // workgroups that share a row, at most
 
 typedef unsigned long long u64;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// What the workgroups of a row hand on, per row.
+struct RowWork {
+    u64 sum[kSteps];
+    u64 near_[kNear];
+    uint32_t count[kSteps];
+    u64 min_sum;
+    uint32_t near_count, unused;
+    float most[kParts], total[kParts], number[kParts];   // of the parts
+};
 
 struct Args {
     const void *logits;
     int64_t row_stride;
     int rows, vocab;
     int bits;           // a weight of 1 is 2^bits
-    float reach;        // (m - l) / temperature beyond which a weight is less than half of 2^-bits
+    int parts;          // workgroups that share a row
+    float near_share;   // of the distance from the mean to the largest logit, within which tokens are kept by themselves
     const float *temperature;
     const int32_t *top_k;
     const float *top_p, *min_p, *uniform;
     int64_t *ids;
     float *logprob;
+    RowWork *work;
 };
 
-// A logit as fp32, NaN as -inf and -0 as +0 (equal logits have equal bits).
-template <typename T>
-__device__ __forceinline__ float logit_of(T raw);
-template <>
-__device__ __forceinline__ float logit_of<float>(float raw) { return raw != raw ? -INFINITY : raw + 0.0f; }
-template <>
-__device__ __forceinline__ float logit_of<_Float16>(_Float16 raw) { return logit_of((float)raw); }
-template <>
-__device__ __forceinline__ float logit_of<uint16_t>(uint16_t raw) { return logit_of(__builtin_bit_cast(float, (uint32_t)raw << 16)); }   // bf16
+// A logit as fp32.
+__device__ __forceinline__ float logit_of(float raw) { return raw; }
+__device__ __forceinline__ float logit_of(_Float16 raw) { return (float)raw; }
+__device__ __forceinline__ float logit_of(uint16_t raw) { return __builtin_bit_cast(float, (uint32_t)raw << 16); }   // bf16
 
-// Larger logits have larger keys.
+// Larger logits have larger keys, equal ones equal ones (-0 is +0).
 __device__ __forceinline__ uint32_t key_of(float l)
 {
-    const uint32_t b = __builtin_bit_cast(uint32_t, l);
+    const uint32_t b = __builtin_bit_cast(uint32_t, l + 0.0f);
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of_key(uint32_t k)
@@ -58,117 +72,217 @@ __device__ __forceinline__ float logit_of_key(uint32_t k)
     return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// exp of x in [-37, 0], by powers of two and the exponential series of what is left (|r| <= ln(2) / 2): terms to r^13, off by 2^-53.
-__device__ __forceinline__ double exponential(double x)
-{
-    const double k = __builtin_rint(x * 1.4426950408889634);
-    const double r = __builtin_fma(k, -0.6931471805599453, x);   // (|k| <= 53: what ln(2) is rounded by comes to 2^-49)
-    double p = 1.0 / 6227020800.0;
-    p = __builtin_fma(p, r, 1.0 / 479001600.0);
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return __builtin_amdgcn_ldexp(p, (int)k);
-}
+constexpr int kFractions = 256;   // of a power of two, in the table of the exponential
+
+struct Table {
+    double power[kFractions];   // 2^(i / 256), by the exponential series
+    constexpr Table() : power()
+    {
+        for (int i = 0; i < kFractions; ++i) {
+            const double x = 0.6931471805599453094 * i / kFractions;
+            double sum = 1.0;
+            for (int n = 24; n > 0; --n) sum = 1.0 + sum * x / n;
+            power[i] = sum;
+        }
+    }
+};
+__device__ const Table kTable;
 
 // What a row's weights are formed with.
 struct Scale {
     float most;        // the largest logit
-    double t, inverse; // the temperature (0 where it is endless) and 1 / temperature
+    double inverse;    // 1 / temperature
+    double fractions;  // 256 log2(e) / temperature
     float steps;       // steps of the histogram per unit of the logit
-    double reach;
     int bits;
-    // the weight, 0 where it is less than half of 2^-bits
-    __device__ __forceinline__ double weight(float l) const
+    int near_steps;    // tokens of earlier steps are kept by themselves
+
+    // The weight as a whole number of 2^-bits; false, and no number, where it is less than half of 2^-bits.  256 log2(e) (l - most) / t = n + f
+    // with |f| <= 1/2; 2^(n / 256) by powers of two and a table, 2^(f / 256) by its series: terms to f^4, off by 2^-54.  Conversions,
+    // roundings and scalings of 64-bit numbers take four times as long as sums and products here, so whole numbers are made by adding
+    // 1.5 * 2^52 (2^52), whose last place is one, and powers of two by adding to the exponent.  (With such instructions and a series of
+    // twelve terms 256 rows of 131072 logits took 187 us.)  NaN has no weight.  (An infinite `most`: it alone has weight.)
+    __device__ __forceinline__ bool weight(float l, const double *table, u64 &w) const
     {
-        if (l == most) return 1.0;
-        const double d = (double)l - (double)most, q = d * inverse;
-        const double x = __builtin_fma(__builtin_fma(-q, t, d), inverse, q);   // d / t
-        return l > -INFINITY && x >= -reach ? exponential(x) : 0.0;            // (an infinite `most`: x is -inf or NaN)
+        if (most == INFINITY) {
+            w = 1ull << bits;
+            return l == most;
+        }
+        const double y = ((double)l - (double)most) * fractions;
+        const double shifted = y + 0x1.8p52;
+        const int n = (int)(uint32_t)__builtin_bit_cast(u64, shifted);
+        const double f = y - (shifted - 0x1.8p52);
+        constexpr double c = 0.6931471805599453 / kFractions;
+        double p = __builtin_fma(f, c * c * c * c / 24.0, c * c * c / 6.0);
+        p = __builtin_fma(p, f, c * c / 2.0);
+        p = __builtin_fma(p, f, c);
+        const double power = table[n & (kFractions - 1)];
+        const double v = __builtin_fma(p * f, power, power);
+        const u64 scaled = __builtin_bit_cast(u64, v) + ((u64)(uint32_t)((n >> 8) + bits) << 52);
+        w = __builtin_bit_cast(u64, __builtin_bit_cast(double, scaled) + 0x1p52) & ((1ull << 52) - 1);
+        return y >= -(double)(kFractions * (bits + 1));
     }
-    __device__ __forceinline__ u64 fixed(double w) const { return (u64)__builtin_rint(__builtin_amdgcn_ldexp(w, bits)); }
-    __device__ __forceinline__ int step(float l) const
-    {
-        return l == most ? 0 : (int)fminf((most - l) * steps, (float)(kSteps - 1));
-    }
+    // The step: larger logits in earlier ones.  (An infinite `most`: all that has weight is in one.)
+    __device__ __forceinline__ float place(float l) const { return (most - l) * steps; }
+    __device__ __forceinline__ int step(float l) const { return (int)fminf(place(l), (float)(kSteps - 1)); }
+    __device__ __forceinline__ double exponent(float l) const { return l == most ? 0.0 : ((double)l - (double)most) * inverse; }
 };
 
-// The element at which a target is reached: its key and index, and the count and sum of the order up to it, itself among them.
+// The element at which a target is reached: its key and index, and the sum of the order up to it, itself among them.
 struct Found {
-    uint32_t key, index, count;
+    uint32_t key, index;
     u64 sum;
 };
 
 struct Shared {
     u64 sum[kSteps];
+    u64 near_[kNear];                              // (key, ~index): in the order where larger comes first
+    u64 member[kMembers], member_weight[kMembers];
     uint32_t count[kSteps];
-    u64 list[kList], list_weight[kList];   // (key, ~index): in the order where larger comes first
+    double table[kFractions];                      // 2^(i / 256)
     u64 wave_sum[kWaves];
     uint32_t wave_count[kWaves];
-    float wave_most[kWaves];
+    float wave_most[kWaves], wave_total[kWaves], wave_number[kWaves];
     u64 digit_sum[256];
     uint32_t digit_count[256];
     int step;
-    uint32_t listed;
+    uint32_t members, near_count;
     Found found;
     u64 before_sum, min_sum;
-    uint32_t before_count, min_count, digit;
+    uint32_t before_count, digit;
 };
 
-template <typename T, typename F>
-__device__ __forceinline__ void for_each(const T *row, int vocab, F f)
+// A row of logits, or a part of it, read by its 16-byte pieces (the first and the last may be part of it only: read by elements).
+template <typename T>
+struct Row {
+    static constexpr int kPiece = 16 / sizeof(T), kAtOnce = 16 / kPiece;
+    const T *first;           // where the piece lies that the row begins in
+    int skip, vocab;
+    int begin, past;          // the pieces of this part
+
+    __device__ __forceinline__ Row(const T *row, int vocab_, int part, int parts) : vocab(vocab_)
+    {
+        skip = (int)(((uintptr_t)row & 15u) / sizeof(T));
+        first = row - skip;
+        const int pieces = (skip + vocab + kPiece - 1) / kPiece, own = (pieces + parts - 1) / parts;
+        begin = min(part * own, pieces);
+        past = min(begin + own, pieces);
+    }
+    __device__ __forceinline__ bool whole(int piece) const { return piece * kPiece >= skip && (piece + 1) * kPiece <= skip + vocab; }
+    __device__ __forceinline__ u32x4 load(int piece) const
+    {
+        if (whole(piece)) return *(const u32x4 *)(first + piece * kPiece);
+        T part[kPiece];
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) {
+            const int i = piece * kPiece + e;
+            part[e] = i >= skip && i < skip + vocab ? first[i] : (T)0;
+        }
+        return __builtin_bit_cast(u32x4, part);
+    }
+    // f(logits of a piece, index of the first): elements outside of the row as -inf
+    template <typename F>
+    __device__ __forceinline__ void visit(int piece, const u32x4 &raw, F f) const
+    {
+        struct Part { T v[kPiece]; };
+        const Part part = __builtin_bit_cast(Part, raw);
+        const int i = piece * kPiece - skip;
+        float l[kPiece];
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) l[e] = logit_of(part.v[e]);
+        if (!whole(piece)) {
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) l[e] = i + e >= 0 && i + e < vocab ? l[e] : -INFINITY;
+        }
+        f(l, i);
+    }
+    template <typename F>
+    __device__ __forceinline__ void raw_pieces(F f) const
+    {
+        for (int p0 = begin + threadIdx.x; p0 < past; p0 += kAtOnce * kThreads) {
+            u32x4 raw[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (p0 + u * kThreads < past) raw[u] = load(p0 + u * kThreads);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (p0 + u * kThreads < past) f(p0 + u * kThreads, raw[u]);
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void by_pieces(F f) const
+    {
+        raw_pieces([&](int piece, const u32x4 &raw) { visit(piece, raw, f); });
+    }
+    template <typename F>
+    __device__ __forceinline__ void for_each(F f) const
+    {
+        by_pieces([&](const float (&l)[kPiece], int i) {
+#pragma unroll
+                for (int e = 0; e < kPiece; ++e) f(l[e], (uint32_t)(i + e));
+        });
+    }
+    __device__ __forceinline__ float at(int i) const { return logit_of(first[skip + i]); }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v)
 {
-    for (int i = threadIdx.x; i < vocab; i += kThreads) f(logit_of(row[i]), (uint32_t)i);
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
 
-// Sums of (count, sum) over the threads before this one; the last thread's own added give the totals.
+// The sum over a wave's lanes up to this one.
+template <typename N>
+__device__ __forceinline__ N wave_scan(N v)
+{
+    auto add = [&](auto ctrl, auto rows) {
+        constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+        if constexpr (sizeof(N) == 8) v += (u64)from_lane<C, R>((uint32_t)(v >> 32)) << 32 | from_lane<C, R>((uint32_t)v);
+        else v += from_lane<C, R>(v);
+    };
+    using std::integral_constant;
+    constexpr integral_constant<int, 0xf> all{};
+    add(integral_constant<int, 0x111>(), all);   // row_shr:1, 2, 4, 8
+    add(integral_constant<int, 0x112>(), all);
+    add(integral_constant<int, 0x114>(), all);
+    add(integral_constant<int, 0x118>(), all);
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());   // row_bcast:15 to rows 1 and 3
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());   // row_bcast:31 to rows 2 and 3
+    return v;
+}
+
+// Sums of (count, sum) over the threads before this one.
 __device__ void exclusive_scan(Shared &s, uint32_t &count, u64 &sum)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t own_count = count;
-    const u64 own_sum = sum;
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t c = __shfl_up(count, d);
-        const u64 w = __shfl_up(sum, d);
-        if (lane >= d) {
-            count += c;
-            sum += w;
-        }
-    }
+    const uint32_t c = wave_scan(count);
+    const u64 w = wave_scan(sum);
     __syncthreads();
     if (lane == 63) {
-        s.wave_count[wave] = count;
-        s.wave_sum[wave] = sum;
+        s.wave_count[wave] = c;
+        s.wave_sum[wave] = w;
     }
     __syncthreads();
-    count -= own_count;
-    sum -= own_sum;
-    for (int w = 0; w < wave; ++w) {
-        count += s.wave_count[w];
-        sum += s.wave_sum[w];
+    count = c - count;
+    sum = w - sum;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        count += i < wave ? s.wave_count[i] : 0;
+        sum += i < wave ? s.wave_sum[i] : 0;
     }
 }
 
 // The first element of the order at which the running count is at least `count` (by_sum false) or the running sum at least `sum`;
 // the row holds one.
-template <typename T>
-__device__ Found reach(Shared &s, const T *row, int vocab, const Scale &scale, bool by_sum, uint32_t count, u64 sum)
+template <typename R>
+__device__ Found reach(Shared &s, const R &row, const Scale &scale, bool by_sum, uint32_t count, u64 sum)
 {
     const int tid = threadIdx.x;
     __syncthreads();
     // the step (the arrays hold running totals)
     for (int i = 0; i < kPerThread; ++i) {
-        const int b = tid * kPerThread + i;
-        const uint32_t c0 = b > 0 ? s.count[b - 1] : 0;
+        const int b = i * kThreads + tid;
+        const uint32_t c0 = !by_sum && b > 0 ? s.count[b - 1] : 0;
         const u64 w0 = b > 0 ? s.sum[b - 1] : 0;
         if (by_sum ? w0 < sum && s.sum[b] >= sum : c0 < count && s.count[b] >= count) {
             s.step = b;
@@ -176,31 +290,104 @@ __device__ Found reach(Shared &s, const T *row, int vocab, const Scale &scale, b
             s.before_sum = w0;
         }
     }
-    if (tid == 0) s.listed = 0;
+    if (tid == 0) s.members = 0;
     __syncthreads();
     const int step = s.step;
     uint32_t before_count = s.before_count;
     u64 before_sum = s.before_sum;
-    if (s.count[step] - before_count <= (uint32_t)kList) {
-        for_each(row, vocab, [&](float l, uint32_t i) {
-            if (scale.step(l) != step) return;
-            const u64 w = scale.fixed(scale.weight(l));
-            if (w == 0) return;
-            const uint32_t at = atomicAdd(&s.listed, 1u);
-            s.list[at] = (u64)key_of(l) << 32 | (uint32_t)~i;
-            s.list_weight[at] = w;
-        });
-        __syncthreads();
-        if (tid < (int)s.listed) {
-            const u64 mine = s.list[tid];
-            uint32_t c = before_count + 1;
-            u64 w = before_sum + s.list_weight[tid];
-            for (uint32_t j = 0; j < s.listed; ++j) {
-                const bool ahead = s.list[j] > mine;
-                c += ahead;
-                w += ahead ? s.list_weight[j] : 0;
+    auto gather = [&](float l, uint32_t i) {
+        u64 w;
+        if (!scale.weight(l, s.table, w) || scale.step(l) != step) return;
+        const uint32_t at = atomicAdd(&s.members, 1u);
+        if (at >= (uint32_t)kMembers) return;
+        s.member[at] = (u64)key_of(l) << 32 | (uint32_t)~i;
+        s.member_weight[at] = w;
+    };
+    if (step < scale.near_steps && s.near_count <= (uint32_t)kNear)
+        for (uint32_t i = tid; i < s.near_count; i += kThreads) gather(logit_of_key((uint32_t)(s.near_[i] >> 32)), (uint32_t)~s.near_[i]);
+    else row.by_pieces([&](const float (&l)[R::kPiece], int i) {
+        // (most pieces hold none: one branch for all of a piece's logits.  The last step holds what lies behind it too, and what an
+        // infinite logit's distance is no number for)
+        bool any = false;
+        const float from = (float)step, past = step == kSteps - 1 ? INFINITY : from + 1.0f;
+#pragma unroll
+        for (int e = 0; e < R::kPiece; ++e) {
+            const float place = scale.place(l[e]);
+            any |= place >= from && place < past;
+        }
+        if (!any && step < kSteps - 1) return;
+#pragma unroll
+        for (int e = 0; e < R::kPiece; ++e) gather(l[e], (uint32_t)(i + e));
+    });
+    __syncthreads();
+    const uint32_t members = s.members;
+    if (members <= (uint32_t)kMembers) {
+        u64 mine = 0, own = 0;
+        int part = -1;
+        if (tid < (int)members) {
+            mine = s.member[tid];
+            own = s.member_weight[tid];
+            part = min((int)((scale.place(logit_of_key((uint32_t)(mine >> 32))) - (float)step) * 256.0f), 255);
+        }
+        uint32_t rivals = members;
+        if (members > 64) {   // a 256th of the step first: each of its members is held against the others
+            if (tid < 256) {
+                s.digit_count[tid] = 0;
+                s.digit_sum[tid] = 0;
             }
-            if (by_sum ? w >= sum && w - s.list_weight[tid] < sum : c == count) s.found = {(uint32_t)(mine >> 32), (uint32_t)~mine, c, w};
+            __syncthreads();
+            if (part >= 0) {
+                atomicAdd(&s.digit_count[part], 1u);
+                atomicAdd(&s.digit_sum[part], own);
+            }
+            if (tid == 0) s.members = 0;
+            __syncthreads();
+            if (tid < 64) {
+                uint32_t c[4];
+                u64 w[4];
+                uint32_t all_c = 0;
+                u64 all_w = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    c[i] = s.digit_count[4 * tid + i];
+                    w[i] = s.digit_sum[4 * tid + i];
+                    all_c += c[i];
+                    all_w += w[i];
+                }
+                uint32_t at_c = before_count + wave_scan(all_c) - all_c;
+                u64 at_w = before_sum + wave_scan(all_w) - all_w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (by_sum ? at_w < sum && at_w + w[i] >= sum : at_c < count && at_c + c[i] >= count) {
+                        s.digit = 4 * tid + i;
+                        s.before_count = at_c;
+                        s.before_sum = at_w;
+                    }
+                    at_c += c[i];
+                    at_w += w[i];
+                }
+            }
+            __syncthreads();
+            before_count = s.before_count;
+            before_sum = s.before_sum;
+            if (part != (int)s.digit) part = -1;
+            if (part >= 0) {
+                const uint32_t at = atomicAdd(&s.members, 1u);
+                s.member[at] = mine;
+                s.member_weight[at] = own;
+            }
+            __syncthreads();
+            rivals = s.members;
+        }
+        if (part >= 0) {
+            uint32_t c = before_count + 1;
+            u64 w = before_sum + own;
+            for (uint32_t j = 0; j < rivals; ++j) {
+                const bool ahead = s.member[j] > mine;
+                c += ahead;
+                w += ahead ? s.member_weight[j] : 0;
+            }
+            if (by_sum ? w >= sum && w - own < sum : c == count) s.found = {(uint32_t)(mine >> 32), (uint32_t)~mine, w};
         }
         __syncthreads();
         return s.found;
@@ -214,11 +401,10 @@ __device__ Found reach(Shared &s, const T *row, int vocab, const Scale &scale, b
             s.digit_sum[tid] = 0;
         }
         __syncthreads();
-        for_each(row, vocab, [&](float l, uint32_t) {
+        row.for_each([&](float l, uint32_t) {
             const uint32_t key = key_of(l);
-            if (scale.step(l) != step || (shift < 24 && key >> (shift + 8) != prefix)) return;
-            const u64 w = scale.fixed(scale.weight(l));
-            if (w == 0) return;
+            u64 w;
+            if (!scale.weight(l, s.table, w) || scale.step(l) != step || (shift < 24 && key >> (shift + 8) != prefix)) return;
             atomicAdd(&s.digit_count[(key >> shift) & 255u], 1u);
             atomicAdd(&s.digit_sum[(key >> shift) & 255u], w);
         });
@@ -240,88 +426,189 @@ __device__ Found reach(Shared &s, const T *row, int vocab, const Scale &scale, b
         before_count = s.before_count;
     }
     // equal logits: the one so many places further on
-    const u64 w = scale.fixed(scale.weight(logit_of_key(prefix)));
+    u64 w;
+    scale.weight(logit_of_key(prefix), s.table, w);
     const uint32_t place = by_sum ? (uint32_t)((sum - before_sum + w - 1) / w) : count - before_count;   // 1 for the first
-    const int own = (vocab + kThreads - 1) / kThreads, first = min(tid * own, vocab), past = min(first + own, vocab);
+    const int own = (row.vocab + kThreads - 1) / kThreads, first = min(tid * own, row.vocab), past = min(first + own, row.vocab);
     uint32_t c = 0;
-    for (int i = first; i < past; ++i) c += key_of(logit_of(row[i])) == prefix;
+    for (int i = first; i < past; ++i) c += key_of(row.at(i)) == prefix;
     uint32_t ahead = c;
     u64 unused = 0;
     exclusive_scan(s, ahead, unused);
     if (ahead < place && ahead + c >= place) {
         uint32_t at = ahead;
         for (int i = first; i < past; ++i)
-            if (key_of(logit_of(row[i])) == prefix && ++at == place) s.found = {prefix, (uint32_t)i, before_count + place, before_sum + place * w};
+            if (key_of(row.at(i)) == prefix && ++at == place) s.found = {prefix, (uint32_t)i, before_sum + place * w};
     }
     __syncthreads();
     return s.found;
 }
 
-// One workgroup per row.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Args a)
-{
-    __shared__ Shared s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x;
-    const T *row = (const T *)a.logits + r * a.row_stride;
+// What is asked of a row.
+struct Asked {
+    float t, p, least;
+    bool greedy;
+    int k;
+    __device__ __forceinline__ Asked(const Args &a, int r)
+    {
+        t = a.temperature ? a.temperature[r] : 1.0f;
+        p = a.top_p ? a.top_p[r] : 1.0f;
+        const float m = a.min_p ? a.min_p[r] : 0.0f;
+        greedy = !(t > 0.0f);
+        k = greedy ? 1 : a.top_k ? a.top_k[r] : 0;
+        least = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
+    }
+};
 
-    float most = -INFINITY;
-    for_each(row, a.vocab, [&](float l, uint32_t) { most = fmaxf(most, l); });
-    for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-    if (lane == 0) s.wave_most[wave] = most;
-    for (int b = tid; b < kSteps; b += kThreads) {
+// `mean`: of the logits that are finite.  (A greedy row: its weights are of no account, the first of its largest logits is.  An
+// endless temperature: all that is not -inf weighs the same.)
+__device__ __forceinline__ Scale scale_of(const Args &a, const Asked &ask, float most, float mean)
+{
+    Scale s;
+    s.most = most;
+    s.inverse = ask.greedy ? 1e30 : ask.t == INFINITY ? 1e-300 : 1.0 / (double)ask.t;
+    s.fractions = s.inverse * (kFractions * 1.4426950408889634);
+    s.steps = ask.greedy ? 1e30f : fminf((float)kSteps / ((a.bits + 1) * 0.6931472f) / ask.t, 1e30f);
+    s.bits = a.bits;
+    const float near_ = (most - mean) * a.near_share * s.steps;
+    s.near_steps = near_ < (float)kSteps ? (int)near_ + 1 : kSteps;
+    return s;
+}
+
+// Over the lanes of a wave: xor 1 and 2 inside quads, the mirrored quad and half of each row of 16, then the four rows.
+template <typename F>
+__device__ __forceinline__ float over_wave(float v, F op)
+{
+    auto other = [](float x, auto ctrl) {
+        const int i = __builtin_bit_cast(int, x);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    v = op(v, other(v, std::integral_constant<int, 0xb1>()));    // quad_perm [1,0,3,2]
+    v = op(v, other(v, std::integral_constant<int, 0x4e>()));    // quad_perm [2,3,0,1]
+    v = op(v, other(v, std::integral_constant<int, 0x141>()));   // row_half_mirror
+    v = op(v, other(v, std::integral_constant<int, 0x140>()));   // row_mirror
+    const int i = __builtin_bit_cast(int, v);
+    auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, lane)); };
+    return op(op(row(0), row(16)), op(row(32), row(48)));
+}
+
+// The largest of a piece's logits (a maximum passes over NaN).
+template <typename T>
+__device__ __forceinline__ float largest_of(const u32x4 &raw)
+{
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 l = __builtin_bit_cast(f32x4, raw);
+        return fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w));
+    } else if constexpr (std::is_same_v<T, _Float16>) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        auto pair = [](uint32_t w) { return __builtin_bit_cast(f16x2, w); };
+        const f16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(pair(raw.x), pair(raw.y)), __builtin_elementwise_max(pair(raw.z), pair(raw.w)));
+        return fmaxf((float)m.x, (float)m.y);
+    } else {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(__builtin_bit_cast(float, raw[i] << 16), __builtin_bit_cast(float, raw[i] & 0xffff0000u)));
+        return m;
+    }
+}
+
+// The largest logit of (a part of) a row, and sum and number of the finite ones among the first of every piece.
+template <typename T>
+__device__ void survey(Shared &s, const Row<T> &row, float &most, float &total, float &number)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    most = -INFINITY;
+    total = number = 0.0f;
+    row.raw_pieces([&](int piece, const u32x4 &raw) {
+        if (row.whole(piece)) {
+            const float first = logit_of(*(const T *)&raw);
+            most = fmaxf(most, largest_of<T>(raw));
+            total += fabsf(first) < INFINITY ? first : 0.0f;
+            number += fabsf(first) < INFINITY ? 1.0f : 0.0f;
+        } else {
+            row.visit(piece, raw, [&](const float (&l)[Row<T>::kPiece], int) {
+#pragma unroll
+                for (int e = 0; e < Row<T>::kPiece; ++e) most = fmaxf(most, l[e]);
+            });
+        }
+    });
+    most = over_wave(most, [](float x, float y) { return fmaxf(x, y); });
+    total = over_wave(total, [](float x, float y) { return x + y; });
+    number = over_wave(number, [](float x, float y) { return x + y; });
+    if (lane == 0) {
+        s.wave_most[wave] = most;
+        s.wave_total[wave] = total;
+        s.wave_number[wave] = number;
+    }
+    __syncthreads();
+    total = number = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        most = fmaxf(most, s.wave_most[w]);
+        total += s.wave_total[w];
+        number += s.wave_number[w];
+    }
+}
+
+__device__ void clear(Shared &s)
+{
+    for (int b = threadIdx.x; b < kSteps; b += kThreads) {
         s.count[b] = 0;
         s.sum[b] = 0;
     }
-    if (tid == 0) {
-        s.min_count = 0;
+    if (threadIdx.x < kFractions) s.table[threadIdx.x] = kTable.power[threadIdx.x];
+    if (threadIdx.x == 0) {
         s.min_sum = 0;
+        s.near_count = 0;
     }
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s.wave_most[w]);
-    if (most == -INFINITY) {
-        if (tid == 0) {
-            a.ids[r] = -1;
-            if (a.logprob) a.logprob[r] = -INFINITY;
-        }
-        return;
-    }
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
-    const bool greedy = !(t > 0.0f);
-    const float p = a.top_p ? a.top_p[r] : 1.0f, asked = a.min_p ? a.min_p[r] : 0.0f;
-    const float least = asked > 0.0f ? fminf(asked, 1.0f) : 0.0f;
-    const int k = greedy ? 1 : a.top_k ? a.top_k[r] : 0;
-    // (a greedy row: its weights are of no account, the first of its largest logits is)
-    const Scale scale = {most, greedy ? 1e-30 : t == INFINITY ? 0.0 : (double)t, greedy ? 1e30 : 1.0 / (double)t,
-                         greedy ? 1e30f : fminf((float)kSteps / a.reach / t, 1e30f), (double)a.reach, a.bits};
+}
 
-    uint32_t min_count = 0;
+// Counts and sums by steps, the tokens near the largest, and the sum of what min_p leaves, of (a part of) a row.
+template <typename T>
+__device__ void histogram(Shared &s, const Row<T> &row, const Scale &scale, const Asked &ask)
+{
     u64 min_sum = 0;
-    for_each(row, a.vocab, [&](float l, uint32_t) {
-        const double w = scale.weight(l);
-        const u64 f = scale.fixed(w);
-        if (f == 0) return;
-        const int b = scale.step(l);
-        atomicAdd(&s.count[b], 1u);
-        atomicAdd(&s.sum[b], f);
-        if (w >= (double)least) {
-            ++min_count;
-            min_sum += f;
+    const u64 min_weight = (u64)__builtin_ceil((double)ask.least * (double)(1ull << scale.bits));
+    row.by_pieces([&](const float (&l)[Row<T>::kPiece], int i) {
+        u64 w[Row<T>::kPiece];
+        bool live[Row<T>::kPiece];
+#pragma unroll
+        for (int e = 0; e < Row<T>::kPiece; ++e) {
+            live[e] = scale.weight(l[e], s.table, w[e]);
+            asm volatile("" : "+v"(w[e]));   // (formed side by side, not each behind a branch of its own)
+        }
+#pragma unroll
+        for (int e = 0; e < Row<T>::kPiece; ++e) {
+            if (!live[e]) continue;
+            const int b = scale.step(l[e]);
+            if (ask.k > 0) atomicAdd(&s.count[b], 1u);   // (counts are asked for by top_k only: the ends of other parts are compared by their sums)
+            atomicAdd(&s.sum[b], w[e]);
+            if (ask.least > 0.0f) min_sum += w[e] >= min_weight ? w[e] : 0;
+            if (b < scale.near_steps) {
+                const uint32_t at = atomicAdd(&s.near_count, 1u);
+                if (at < (uint32_t)kNear) s.near_[at] = (u64)key_of(l[e]) << 32 | (uint32_t)~(uint32_t)(i + e);
+            }
         }
     });
-    if (least > 0.0f) {
-        atomicAdd(&s.min_count, min_count);
-        atomicAdd(&s.min_sum, min_sum);
-    }
+    if (ask.least > 0.0f) atomicAdd(&s.min_sum, min_sum);
+}
+
+// The token, from the histogram of the whole row.
+template <typename T>
+__device__ void choose(const Args &a, Shared &s, const Row<T> &row, const Scale &scale, const Asked &ask, int r)
+{
+    const int tid = threadIdx.x;
     __syncthreads();
     {   // running totals
         uint32_t c = 0;
         u64 w = 0;
+#pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
             c += s.count[tid * kPerThread + i];
             w += s.sum[tid * kPerThread + i];
         }
         exclusive_scan(s, c, w);
+#pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
             c += s.count[tid * kPerThread + i];
             w += s.sum[tid * kPerThread + i];
@@ -330,40 +617,161 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a)
         }
     }
     __syncthreads();
-    uint32_t kept = s.count[kSteps - 1];
     u64 total = s.sum[kSteps - 1];
-    if (k > 0 && (uint32_t)k < kept) {
-        const Found f = reach(s, row, a.vocab, scale, false, (uint32_t)k, 0);
-        kept = f.count;
-        total = f.sum;
+    if (ask.k > 0 && (uint32_t)ask.k < s.count[kSteps - 1]) total = reach(s, row, scale, false, (uint32_t)ask.k, 0).sum;
+    if (ask.p < 1.0f) {
+        const double target = __builtin_ceil((double)fmaxf(ask.p, 0.0f) * (double)total);
+        total = min(total, reach(s, row, scale, true, 0, target < 1.0 ? 1 : (u64)target).sum);
     }
-    if (p < 1.0f && kept > 1) {
-        const double target = __builtin_ceil((double)fmaxf(p, 0.0f) * (double)total);
-        const Found f = reach(s, row, a.vocab, scale, true, 0, target < 1.0 ? 1 : (u64)target);
-        if (f.count < kept) {
-            kept = f.count;
-            total = f.sum;
-        }
-    }
-    if (least > 0.0f && s.min_count < kept) {
-        kept = s.min_count;
-        total = s.min_sum;
-    }
+    if (ask.least > 0.0f) total = min(total, s.min_sum);
     float u = a.uniform[r];
     u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
     u64 target = (u64)__builtin_floor((double)u * (double)total);
     if (target >= total) target = total - 1;
-    const Found f = reach(s, row, a.vocab, scale, true, 0, target + 1);
+    const Found f = reach(s, row, scale, true, 0, target + 1);
     if (tid == 0) {
         a.ids[r] = f.index;
-        if (a.logprob) a.logprob[r] = kept == 1 ? 0.0f : (float)log(scale.weight(logit_of_key(f.key)) * (double)(1ull << a.bits) / (double)total);
+        if (a.logprob) a.logprob[r] = ask.greedy ? 0.0f : (float)(scale.exponent(logit_of_key(f.key)) - log((double)total / (double)(1ull << a.bits)));
     }
+}
+
+__device__ __forceinline__ void nothing(const Args &a, int r)
+{
+    if (threadIdx.x != 0) return;
+    a.ids[r] = -1;
+    if (a.logprob) a.logprob[r] = -INFINITY;
+}
+
+// One workgroup per row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const Args a)
+{
+    __shared__ Shared s;
+    const int r = blockIdx.x;
+    const Row<T> row((const T *)a.logits + r * a.row_stride, a.vocab, 0, 1);
+    const Asked ask(a, r);
+    clear(s);
+    float most, total, number;
+    survey(s, row, most, total, number);
+    if (most == -INFINITY) return nothing(a, r);
+    const Scale scale = scale_of(a, ask, most, total / number);
+    histogram(s, row, scale, ask);
+    choose(a, s, row, scale, ask, r);
+}
+
+// The same by several workgroups a row, where rows are few: a launch that looks for the largest logit (and clears what the next one
+// adds to), one that adds up histograms, one that chooses.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) survey_kernel(const Args a)
+{
+    __shared__ Shared s;
+    const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    RowWork &work = a.work[r];
+    const Row<T> row((const T *)a.logits + r * a.row_stride, a.vocab, part, a.parts);
+    for (int b = part * kThreads + threadIdx.x; b < kSteps; b += a.parts * kThreads) {
+        work.sum[b] = 0;
+        work.count[b] = 0;
+    }
+    float most, total, number;
+    survey(s, row, most, total, number);
+    if (threadIdx.x != 0) return;
+    work.most[part] = most;
+    work.total[part] = total;
+    work.number[part] = number;
+    if (part == 0) {
+        work.min_sum = 0;
+        work.near_count = 0;
+    }
+}
+
+__device__ __forceinline__ bool scale_of_row(const Args &a, const Asked &ask, const RowWork &work, Scale &scale)
+{
+    float most = -INFINITY, total = 0.0f, number = 0.0f;
+    for (int i = 0; i < a.parts; ++i) {
+        most = fmaxf(most, work.most[i]);
+        total += work.total[i];
+        number += work.number[i];
+    }
+    scale = scale_of(a, ask, most, total / number);
+    return most > -INFINITY;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) histogram_kernel(const Args a)
+{
+    __shared__ Shared s;
+    const int tid = threadIdx.x, r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    RowWork &work = a.work[r];
+    const Row<T> row((const T *)a.logits + r * a.row_stride, a.vocab, part, a.parts);
+    const Asked ask(a, r);
+    Scale scale;
+    if (!scale_of_row(a, ask, work, scale)) return;
+    clear(s);
+    __syncthreads();
+    histogram(s, row, scale, ask);
+    __syncthreads();
+    for (int b = tid; b < kSteps; b += kThreads) {
+        const u64 w = s.sum[b];
+        if (w) atomicAdd(&work.sum[b], w);
+        const uint32_t c = s.count[b];
+        if (c) atomicAdd(&work.count[b], c);
+    }
+    const uint32_t own = s.near_count;
+    if (tid == 0) {
+        s.members = own ? atomicAdd(&work.near_count, own) : 0;
+        if (s.min_sum) atomicAdd(&work.min_sum, s.min_sum);
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < own && s.members + i < (uint32_t)kNear && i < (uint32_t)kNear; i += kThreads) work.near_[s.members + i] = s.near_[i];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) choose_kernel(const Args a)
+{
+    __shared__ Shared s;
+    const int tid = threadIdx.x, r = blockIdx.x;
+    const RowWork &work = a.work[r];
+    const Row<T> row((const T *)a.logits + r * a.row_stride, a.vocab, 0, 1);
+    const Asked ask(a, r);
+    Scale scale;
+    if (!scale_of_row(a, ask, work, scale)) return nothing(a, r);
+    for (int b = tid; b < kSteps; b += kThreads) {
+        s.sum[b] = work.sum[b];
+        s.count[b] = work.count[b];
+    }
+    const uint32_t listed = work.near_count;
+    if (listed <= (uint32_t)kNear)
+        for (uint32_t i = tid; i < listed; i += kThreads) s.near_[i] = work.near_[i];
+    if (tid < kFractions) s.table[tid] = kTable.power[tid];
+    if (tid == 0) {
+        s.near_count = listed;
+        s.min_sum = work.min_sum;
+    }
+    choose(a, s, row, scale, ask, r);
 }
 
 int launch_status()
 {
     hipError_t e = hipGetLastError();
     return e == hipSuccess ? LUTGEMM_OK : lutgemm_internal_hip_fail((int)e);
+}
+
+// Tokens within this share of the distance from the mean logit to the largest are kept by themselves, so that a target that
+// is reached among them needs no further look at the row: for normally distributed logits some 2000 of them (half the room there is).
+float near_share(int vocab)
+{
+    return vocab <= 8000 ? 1.0f : 1.0f - sqrtf(logf(vocab / 8000.0f) / logf((float)vocab));
+}
+
+// Workgroups that share a row, in three launches instead of one: where rows leave CUs idle and are long enough to pay for the two more
+// launches, and for the addition of histograms, which takes longer the more of them there are.  One row of 131072 logits 64.6 -> 36.4 us with
+// 8 (32 parts 33.1, but 8 rows of 50272 28.9 instead of 26.0), 128 rows 84.6 -> 77.2 with 2, 8 rows of 50272 36.0 -> 30.8; one of 32000 24.4 -> 23.3
+// with 7 without filters, 31.9 -> 30.3 with all, 64 rows of 50272 38.2 -> 37.4 with 4: not worth them.
+int parts_of(int rows, int vocab)
+{
+    if (vocab < 40000 || (rows > 32 && vocab < 80000)) return 1;
+    const int parts = 256 / rows;
+    return parts > 8 ? 8 : parts < 1 ? 1 : parts;
 }
 
 bool sizes_fit(int rows, int vocab) { return rows >= 1 && rows <= 65535 && vocab >= 1 && vocab <= 1 << 20; }
@@ -374,7 +782,8 @@ extern "C" {
 
 size_t lutgemm_sampling_workspace(int rows, int vocab)
 {
-    return sizes_fit(rows, vocab) ? 16 : 0;
+    if (!sizes_fit(rows, vocab)) return 0;
+    return parts_of(rows, vocab) > 1 ? rows * sizeof(RowWork) : 16;
 }
 
 int lutgemm_sample_tokens(const lutgemm_sampling *c, void *workspace, size_t workspace_bytes, void *stream)
@@ -389,14 +798,43 @@ int lutgemm_sample_tokens(const lutgemm_sampling *c, void *workspace, size_t wor
         return LUTGEMM_EALIGN;
     int doublings = 0;
     while (1 << doublings < c->vocab) ++doublings;
-    const int bits = 63 - doublings < 52 ? 63 - doublings : 52;
-    const Args a = {c->logits, c->row_stride, c->rows, c->vocab, bits, (bits + 1) * 0.6931472f, c->temperature, c->top_k, c->top_p, c->min_p, c->uniform, c->ids, c->logprob};
+    const int bits = 63 - doublings < 51 ? 63 - doublings : 51;
+    Args a{};
+    a.logits = c->logits;
+    a.row_stride = c->row_stride;
+    a.rows = c->rows;
+    a.vocab = c->vocab;
+    a.bits = bits;
+    a.parts = parts_of(c->rows, c->vocab);
+    a.near_share = near_share(c->vocab);
+    a.temperature = c->temperature;
+    a.top_k = c->top_k;
+    a.top_p = c->top_p;
+    a.min_p = c->min_p;
+    a.uniform = c->uniform;
+    a.ids = c->ids;
+    a.logprob = c->logprob;
+    a.work = (RowWork *)workspace;
     const hipStream_t hs = (hipStream_t)stream;
-    const dim3 grid((unsigned)c->rows), threads(kThreads);
-    if (c->logits_type == LUTGEMM_TYPE_F16) hipLaunchKernelGGL(sample_kernel<_Float16>, grid, threads, 0, hs, a);
-    else if (c->logits_type == LUTGEMM_TYPE_BF16) hipLaunchKernelGGL(sample_kernel<uint16_t>, grid, threads, 0, hs, a);
-    else hipLaunchKernelGGL(sample_kernel<float>, grid, threads, 0, hs, a);
-    return launch_status();
+    auto launch = [&](auto type) {
+        typedef decltype(type) T;
+        const dim3 rows((unsigned)c->rows), parts((unsigned)(c->rows * a.parts)), threads(kThreads);
+        if (a.parts == 1) {
+            hipLaunchKernelGGL(sample_kernel<T>, rows, threads, 0, hs, a);
+            return launch_status();
+        }
+        hipLaunchKernelGGL(survey_kernel<T>, parts, threads, 0, hs, a);
+        int status = launch_status();
+        if (status != LUTGEMM_OK) return status;
+        hipLaunchKernelGGL(histogram_kernel<T>, parts, threads, 0, hs, a);
+        status = launch_status();
+        if (status != LUTGEMM_OK) return status;
+        hipLaunchKernelGGL(choose_kernel<T>, rows, threads, 0, hs, a);
+        return launch_status();
+    };
+    if (c->logits_type == LUTGEMM_TYPE_F16) return launch(_Float16());
+    if (c->logits_type == LUTGEMM_TYPE_BF16) return launch(uint16_t());
+    return launch(float());
 }
 
 }  // extern "C"
