@@ -169,20 +169,48 @@ struct Row {
         past = min(begin + own, pieces);
     }
     __device__ __forceinline__ bool whole(int piece) const { return piece * kPiece >= skip && (piece + 1) * kPiece <= skip + vocab; }
-    __device__ __forceinline__ u32x4 load(int piece) const
+    // f(piece, its 16 bytes, whether all of them are the row's): whole pieces, several at a time, then what the row's ends have of theirs.
+    template <typename F>
+    __device__ __forceinline__ void raw_pieces(F f) const
     {
-        if (whole(piece)) return *(const u32x4 *)(first + piece * kPiece);
-        T part[kPiece];
+        if (begin == past) return;
+        const int from = begin + (whole(begin) ? 0 : 1), to = past - (whole(past - 1) ? 0 : 1);
+        const u32x4 *pieces = (const u32x4 *)first;
+        int p0 = from + threadIdx.x, end = threadIdx.x == 0 && from > begin ? begin : threadIdx.x == 1 && to < past && past - 1 > begin ? past - 1 : -1;
+        // (a row of one piece that is not whole: the first thread's)
+        if (past - 1 == begin && threadIdx.x == 1) end = -1;
+        while (true) {
+            u32x4 raw[kAtOnce];
+            int number = 0, base = p0;
+            const bool inside = p0 < to;
+            if (inside) {
+                number = min((to - p0 + kThreads - 1) / kThreads, kAtOnce);
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) {
-            const int i = piece * kPiece + e;
-            part[e] = i >= skip && i < skip + vocab ? first[i] : (T)0;
+                for (int u = 0; u < kAtOnce; ++u)
+                    if (u < number) raw[u] = pieces[p0 + u * kThreads];
+                p0 += kAtOnce * kThreads;
+            } else if (end >= 0) {
+                T part[kPiece];
+#pragma unroll
+                for (int e = 0; e < kPiece; ++e) {
+                    const int i = end * kPiece + e;
+                    part[e] = i >= skip && i < skip + vocab ? first[i] : (T)0;
+                }
+                raw[0] = __builtin_bit_cast(u32x4, part);
+                number = 1;
+                base = end;
+                end = -1;
+            } else {
+                break;
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (u < number) f(base + u * kThreads, raw[u], inside);
         }
-        return __builtin_bit_cast(u32x4, part);
     }
     // f(logits of a piece, index of the first): elements outside of the row as -inf
     template <typename F>
-    __device__ __forceinline__ void visit(int piece, const u32x4 &raw, F f) const
+    __device__ __forceinline__ void visit(int piece, const u32x4 &raw, bool inside, F f) const
     {
         struct Part { T v[kPiece]; };
         const Part part = __builtin_bit_cast(Part, raw);
@@ -190,29 +218,16 @@ struct Row {
         float l[kPiece];
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) l[e] = logit_of(part.v[e]);
-        if (!whole(piece)) {
+        if (!inside) {
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) l[e] = i + e >= 0 && i + e < vocab ? l[e] : -INFINITY;
         }
         f(l, i);
     }
     template <typename F>
-    __device__ __forceinline__ void raw_pieces(F f) const
-    {
-        for (int p0 = begin + threadIdx.x; p0 < past; p0 += kAtOnce * kThreads) {
-            u32x4 raw[kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                if (p0 + u * kThreads < past) raw[u] = load(p0 + u * kThreads);
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-                if (p0 + u * kThreads < past) f(p0 + u * kThreads, raw[u]);
-        }
-    }
-    template <typename F>
     __device__ __forceinline__ void by_pieces(F f) const
     {
-        raw_pieces([&](int piece, const u32x4 &raw) { visit(piece, raw, f); });
+        raw_pieces([&](int piece, const u32x4 &raw, bool inside) { visit(piece, raw, inside, f); });
     }
     template <typename F>
     __device__ __forceinline__ void for_each(F f) const
@@ -519,14 +534,14 @@ __device__ void survey(Shared &s, const Row<T> &row, float &most, float &total, 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     most = -INFINITY;
     total = number = 0.0f;
-    row.raw_pieces([&](int piece, const u32x4 &raw) {
-        if (row.whole(piece)) {
+    row.raw_pieces([&](int piece, const u32x4 &raw, bool inside) {
+        if (inside) {
             const float first = logit_of(*(const T *)&raw);
             most = fmaxf(most, largest_of<T>(raw));
             total += fabsf(first) < INFINITY ? first : 0.0f;
             number += fabsf(first) < INFINITY ? 1.0f : 0.0f;
         } else {
-            row.visit(piece, raw, [&](const float (&l)[Row<T>::kPiece], int) {
+            row.visit(piece, raw, false, [&](const float (&l)[Row<T>::kPiece], int) {
 #pragma unroll
                 for (int e = 0; e < Row<T>::kPiece; ++e) most = fmaxf(most, l[e]);
             });
