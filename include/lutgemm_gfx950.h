@@ -779,12 +779,13 @@ int lutgemm_sample_tokens(const lutgemm_sampling *call, void *workspace, size_t 
  *   ids int32 [M], device;  down fp16 [adapters][rank][K], up fp16 [adapters][N][rank], 16-byte aligned;  scale float
  *   [adapters], or NULL (1)
  *   K % 32 == 0, N % 4 == 0, rank % 8 == 0, 8 <= rank <= 256 (adapters of other or unlike ranks are filled up with zeros),
- *   1 <= M <= 65535, 1 <= adapters <= 65535
+ *   1 <= M <= 65535, 1 <= adapters <= LUTGEMM_MAX_ADAPTERS
  * Several layers of one call (projections that share their input, or do not) share its launches: 1 <= count <=
  * LUTGEMM_MAX_GROUP.  What one of them writes may not overlap what another reads or writes.
  * `workspace`: lutgemm_adapters_workspace bytes (0 for arguments that are refused), 16-byte aligned, of any contents, in use until
  * the call's work is done.
  */
+#define LUTGEMM_MAX_ADAPTERS 8192
 typedef struct lutgemm_adapters {
     const void *x_f16, *base_f16;
     void *out_f16;

@@ -1,8 +1,20 @@
 // Low-rank adapters of many requests beside a shared linear layer, gfx950: out = base + scale * up (down x), every row through the
-// adapter that its id names.  Two launches: down, which leaves h = down x in fp32, and up.
+// adapter that its id names.
+//
+// Rows of one adapter are taken together, up to 16 of them, which are the columns of the matrix instruction in both products:
+//   h^T = down x^T      A: 16 ranks of down, B: 16 rows of x.  The waves of a workgroup, and workgroups, share K; parts of h are
+//                       left side by side in fp32 and added up, in their order, by the next launch.
+//   out^T = up h^T      A: 16 outputs of up, B: the rows' h.  h keeps its 32 bits: a row is scaled by a power of two to at most 1 and
+//                       held as the sum of two fp16 numbers, 2^-25 of its largest apart from it, which the instruction multiplies one
+//                       after the other.
+// A column of the instruction depends on nothing but its own row, so what rows stand beside it makes no difference to a result.
+// Bound by reading the adapters that are used (few rows), or x, base and out (many).  Up to 256 rows every workgroup finds by
+// itself which rows share its row's adapter; more rows are sorted by a launch ahead.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "lutgemm_gfx950.h"
 #include "lutgemm_common.h"
@@ -16,6 +28,16 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kTile = 16;              // rows taken together
+constexpr int kUnsorted = 256;         // rows up to which workgroups look for their own
+constexpr int kMaxAdapters = LUTGEMM_MAX_ADAPTERS;
+constexpr int kDepth = 128;            // inputs a wave takes at a time
+constexpr int kColumns = 64;           // outputs a wave takes at a time
+
+// Rows of one adapter: `count` entries of the order from `first` on.
+struct Tile {
+    int id, first, count;
+};
 
 struct Problem {
     const _Float16 *x, *base;
@@ -25,7 +47,12 @@ struct Problem {
     const float *scale;
     int64_t x_stride, base_stride, out_stride;
     int M, N, K, rank, adapters;
-    float *h;   // [M][rank]
+    int slots;                 // tiles there can be: workgroups that look for rows
+    int k_splits, k_own;       // workgroups that share K, and the inputs each takes (a multiple of kDepth)
+    int n_own;                 // outputs a workgroup takes
+    float *h;                  // [k_splits][M][rank]
+    Tile *tiles;               // sorted rows: the tiles (a count of 0 behind the last), and
+    int32_t *order;            // the rows
 };
 
 struct Args {
@@ -33,56 +60,252 @@ struct Args {
     Problem p[LUTGEMM_MAX_GROUP];
 };
 
-// One workgroup per row: the waves take the ranks in turn.
+// The adapter of a row, or -1.
+__device__ __forceinline__ int adapter_of(const Problem &p, int m)
+{
+    const int id = p.ids[m];
+    return id >= 0 && id < p.adapters ? id : -1;
+}
+
+// The rows of this slot's tile: their number (0: none) and, in `rows`, which; `id` their adapter, -1 for rows without one.
+__device__ int rows_of(const Problem &p, int slot, int (&rows)[kTile], unsigned long long (&alike)[kWaves], int &id)
+{
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (p.order) {
+        const Tile tile = p.tiles[slot];
+        id = tile.id;
+        if (tid < tile.count) rows[tid] = p.order[tile.first + tid];
+        __syncthreads();
+        return tile.count;
+    }
+    // the first, 17th, ... row of an adapter's takes its next 16
+    id = adapter_of(p, slot);
+    const bool mine = tid < p.M && adapter_of(p, tid) == id;
+    const unsigned long long ballot = __ballot(mine);
+    if (lane == 0) alike[wave] = ballot;
+    __syncthreads();
+    int ahead = 0, before_slot = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const unsigned long long b = alike[w];
+        all += __popcll(b);
+        ahead += w < wave ? __popcll(b) : w == wave ? __popcll(b & ((1ull << lane) - 1)) : 0;
+        before_slot += w < slot >> 6 ? __popcll(b) : w == slot >> 6 ? __popcll(b & ((1ull << (slot & 63)) - 1)) : 0;
+    }
+    if (before_slot % kTile != 0) return 0;
+    const int place = ahead - before_slot;
+    if (mine && place >= 0 && place < kTile) rows[place] = tid;
+    __syncthreads();
+    return min(all - before_slot, kTile);
+}
+
+// Sorts the rows of a problem by adapter (rows without one last) and cuts them into tiles.  One workgroup; the order of an adapter's rows is
+// any, which makes no difference to results.
+__global__ void __launch_bounds__(1024) sort_kernel(const Args args)
+{
+    constexpr int kOwn = (kMaxAdapters + 1 + 1023) / 1024;
+    __shared__ int rows[kMaxAdapters + 1];
+    __shared__ int wave_rows[16], wave_tiles[16];
+    const Problem &p = args.p[blockIdx.x];
+    if (!p.order) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kinds = p.adapters + 1;
+    for (int a = tid; a < kinds; a += 1024) rows[a] = 0;
+    __syncthreads();
+    auto kind_of = [&](int m) {
+        const int id = adapter_of(p, m);
+        return id < 0 ? p.adapters : id;
+    };
+    for (int m = tid; m < p.M; m += 1024) atomicAdd(&rows[kind_of(m)], 1);
+    __syncthreads();
+    int own[kOwn], own_rows = 0, own_tiles = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const int a = tid * kOwn + i;
+        own[i] = a < kinds ? rows[a] : 0;
+        own_rows += own[i];
+        own_tiles += (own[i] + kTile - 1) / kTile;
+    }
+    int to_rows = own_rows, to_tiles = own_tiles;
+    for (int d = 1; d < 64; d *= 2) {
+        const int r = __shfl_up(to_rows, d), t = __shfl_up(to_tiles, d);
+        to_rows += lane >= d ? r : 0;
+        to_tiles += lane >= d ? t : 0;
+    }
+    if (lane == 63) {
+        wave_rows[wave] = to_rows;
+        wave_tiles[wave] = to_tiles;
+    }
+    __syncthreads();
+    int first = to_rows - own_rows, tile = to_tiles - own_tiles, tiles = 0;
+    for (int w = 0; w < 16; ++w) {
+        first += w < wave ? wave_rows[w] : 0;
+        tile += w < wave ? wave_tiles[w] : 0;
+        tiles += wave_tiles[w];
+    }
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const int a = tid * kOwn + i;
+        if (a >= kinds) break;
+        rows[a] = first;   // (from here on: where the adapter's next row goes)
+        for (int r = 0; r < own[i]; r += kTile) p.tiles[tile++] = {a < p.adapters ? a : -1, first + r, min(own[i] - r, kTile)};
+        first += own[i];
+    }
+    for (int t = tiles + tid; t < p.slots; t += 1024) p.tiles[t] = {-1, 0, 0};
+    __syncthreads();
+    for (int m = tid; m < p.M; m += 1024) p.order[atomicAdd(&rows[kind_of(m)], 1)] = m;
+}
+
+// A part of h for the rows of a tile.  A wave takes 128 inputs at a time, a lane 32 of them side by side (64 bytes of a row of x and of
+// each row of down), eight for each instruction: the inputs are summed over in any order, as long as both operands keep it.
+template <int NT>   // tiles of 16 ranks, at least as many as there are
 __global__ void __launch_bounds__(kThreads) down_kernel(const Args args)
 {
-    const Problem &p = args.p[blockIdx.y];
-    const int m = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    if (m >= p.M) return;
-    const int id = p.ids[m];
-    if (id < 0 || id >= p.adapters) return;
-    const _Float16 *x = p.x + m * p.x_stride;
-    for (int r = wave; r < p.rank; r += kWaves) {
-        const _Float16 *row = p.down + ((size_t)id * p.rank + r) * p.K;
-        float sum = 0.0f;
-        for (int k = lane * 8; k < p.K; k += 512) {
-            const f16x8 xv = *(const f16x8 *)(x + k), wv = *(const f16x8 *)(row + k);
+    __shared__ float parts[kWaves][NT * 16][kTile + 1];
+    __shared__ int rows[kTile];
+    __shared__ unsigned long long alike[kWaves];
+    const Problem &p = args.p[blockIdx.z];
+    const int slot = blockIdx.x, split = blockIdx.y;
+    if (slot >= p.slots || split >= p.k_splits) return;
+    int id;
+    const int count = rows_of(p, slot, rows, alike, id);
+    if (count == 0 || id < 0) return;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, column = lane & 15, quad = lane >> 4;
+    const _Float16 *x = p.x + rows[min(column, count - 1)] * p.x_stride;
+    const _Float16 *down = p.down + (size_t)id * p.rank * p.K;
+    const int from = split * p.k_own, to = min(from + p.k_own, p.K), rank_tiles = (p.rank + 15) / 16;
+    f32x4 acc[NT];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf((float)xv[i], (float)wv[i], sum);
+    for (int t = 0; t < NT; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = from + wave * kDepth; k0 < to; k0 += kWaves * kDepth) {
+        const int k = k0 + quad * 32;
+        const bool inside = k < p.K;   // (a lane's 32 inputs are there or not, all of them)
+        f16x8 xv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xv[i] = inside ? *(const f16x8 *)(x + k + 8 * i) : (f16x8)((_Float16)0.0f);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (t < rank_tiles) {
+                const _Float16 *row = down + (size_t)min(16 * t + column, p.rank - 1) * p.K + k;
+                f16x8 dv[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dv[i] = inside ? *(const f16x8 *)(row + 8 * i) : (f16x8)((_Float16)0.0f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dv[i], xv[i], acc[t], 0, 0, 0);
+            }
         }
-        for (int s = 1; s < 64; s *= 2) sum += __shfl_xor(sum, s);
-        if (lane == 0) p.h[(size_t)m * p.rank + r] = sum;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) parts[wave][16 * t + 4 * quad + i][column] = acc[t][i];
+    __syncthreads();
+    float *h = p.h + (size_t)split * p.M * p.rank;
+    for (int u = tid; u < count * p.rank; u += kThreads) {
+        const int row = u / p.rank, r = u % p.rank;
+        float sum = parts[0][r][row];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += parts[w][r][row];
+        h[(size_t)rows[row] * p.rank + r] = sum;
     }
 }
 
-// One thread per four outputs of a row.
+// out for the rows of a tile and some outputs.  A wave takes 64 outputs at a time in four instructions, whose 16 outputs are dealt out so
+// that a lane ends up with 16 neighbouring ones of its row.
+template <int RT>   // steps of 32 ranks, at least as many as there are
 __global__ void __launch_bounds__(kThreads) up_kernel(const Args args)
 {
+    constexpr int kPadded = RT * 32 + 8;
+    __shared__ _Float16 high[kTile][kPadded], low[kTile][kPadded];
+    __shared__ float back[kTile];   // what a row's sums are multiplied by
+    __shared__ int rows[kTile];
+    __shared__ unsigned long long alike[kWaves];
     const Problem &p = args.p[blockIdx.z];
-    const int m = blockIdx.y, n = (blockIdx.x * kThreads + threadIdx.x) * 4;
-    if (m >= p.M || n >= p.N) return;
-    const f16x4 base = *(const f16x4 *)(p.base + m * p.base_stride + n);
-    f16x4 *out = (f16x4 *)(p.out + m * p.out_stride + n);
-    const int id = p.ids[m];
-    if (id < 0 || id >= p.adapters) {
-        *out = base;
+    const int slot = blockIdx.x, from = blockIdx.y * p.n_own;
+    if (slot >= p.slots || from >= p.N) return;
+    const int to = min(from + p.n_own, p.N);
+    int id;
+    const int count = rows_of(p, slot, rows, alike, id);
+    if (count == 0) return;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, column = lane & 15, quad = lane >> 4;
+    if (id < 0) {
+        if (p.out == p.base) return;
+        const int fours = (to - from) / 4;
+        for (int u = tid; u < count * fours; u += kThreads) {
+            const int m = rows[u / fours], n = from + u % fours * 4;
+            *(f16x4 *)(p.out + m * p.out_stride + n) = *(const f16x4 *)(p.base + m * p.base_stride + n);
+        }
         return;
     }
-    const float *h = p.h + (size_t)m * p.rank;
-    const _Float16 *up = p.up + ((size_t)id * p.N + n) * p.rank;
-    const float scale = p.scale ? p.scale[id] : 1.0f;
-    f16x4 result;
+    {   // h of the rows: 16 threads each
+        const int row = tid / 16, part = tid % 16;
+        const bool live = row < count;
+        const float *h = p.h + (size_t)rows[live ? row : 0] * p.rank;
+        float v[RT * 2], most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float sum = 0.0f;
-        for (int r = 0; r < p.rank; r += 8) {
-            const f16x8 u = *(const f16x8 *)(up + (size_t)i * p.rank + r);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf((float)u[j], h[r + j], sum);
+        for (int i = 0; i < RT * 2; ++i) {
+            const int r = part + 16 * i;
+            v[i] = 0.0f;
+            if (r < p.rank && live) {
+#pragma unroll 4
+                for (int s = 0; s < p.k_splits; ++s) v[i] += h[(size_t)s * p.M * p.rank + r];
+            }
+            most = fmaxf(most, fabsf(v[i]));
         }
-        result[i] = (_Float16)((float)base[i] + scale * sum);
+#pragma unroll
+        for (int m = 1; m < 16; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+        // (a power of two not below the largest, inside what can be inverted; infinite rows stay as they are)
+        const int exponent = most > 0.0f && most < INFINITY ? min(max(__builtin_amdgcn_frexp_expf(most), -100), 100) : 0;
+#pragma unroll
+        for (int i = 0; i < RT * 2; ++i) {
+            const float scaled = __builtin_amdgcn_ldexpf(v[i], -exponent);
+            const _Float16 hi = (_Float16)scaled;
+            high[row][part + 16 * i] = hi;
+            low[row][part + 16 * i] = (_Float16)(scaled - (float)hi);
+        }
+        if (part == 0) back[row] = __builtin_amdgcn_ldexpf(p.scale ? p.scale[id] : 1.0f, exponent);
     }
-    *out = result;
+    __syncthreads();
+    f16x8 hi[RT], lo[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        hi[t] = *(const f16x8 *)&high[column][32 * t + 8 * quad];
+        lo[t] = *(const f16x8 *)&low[column][32 * t + 8 * quad];
+    }
+    const float scale = back[column];
+    const int m = rows[min(column, count - 1)];
+    const _Float16 *base = p.base + m * p.base_stride;
+    _Float16 *out = p.out + m * p.out_stride;
+    const _Float16 *up = p.up + (size_t)id * p.N * p.rank;
+    for (int n0 = from + wave * kColumns; n0 < to; n0 += kWaves * kColumns) {
+        f32x4 acc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            // instruction t's row `column` is output (column / 4) * 16 + 4 t + column % 4
+            const int n = min(n0 + column / 4 * 16 + 4 * t + column % 4, p.N - 1);
+            const _Float16 *row = up + (size_t)n * p.rank;
+#pragma unroll
+            for (int s = 0; s < RT; ++s) {
+                if (32 * s < p.rank) {
+                    const int r = 32 * s + 8 * quad;
+                    const f16x8 u = r < p.rank ? *(const f16x8 *)(row + r) : (f16x8)((_Float16)0.0f);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, hi[s], acc[t], 0, 0, 0);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, lo[s], acc[t], 0, 0, 0);
+                }
+            }
+        }
+        if (column >= count) continue;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int n = n0 + 16 * quad + 4 * t;
+            if (n >= to) continue;
+            const f16x4 b = *(const f16x4 *)(base + n);
+            f16x4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = (_Float16)fmaf(acc[t][i], scale, (float)b[i]);
+            *(f16x4 *)(out + n) = o;
+        }
+    }
 }
 
 int launch_status()
@@ -112,7 +335,7 @@ int check(int count, const lutgemm_adapters *ps)
         const lutgemm_adapters &p = ps[i];
         if (!p.x_f16 || !p.base_f16 || !p.out_f16 || !p.ids || !p.down_f16 || !p.up_f16) return LUTGEMM_EINVAL;
         if (p.M < 1 || p.M > 65535 || p.K < 32 || p.K % 32 != 0 || p.K > 1 << 20 || p.N < 4 || p.N % 4 != 0 || p.N > 1 << 20) return LUTGEMM_EINVAL;
-        if (p.rank < 8 || p.rank > 256 || p.rank % 8 != 0 || p.adapters < 1 || p.adapters > 65535) return LUTGEMM_EINVAL;
+        if (p.rank < 8 || p.rank > 256 || p.rank % 8 != 0 || p.adapters < 1 || p.adapters > kMaxAdapters) return LUTGEMM_EINVAL;
         if (p.M > 1 && (p.x_stride < 0 || p.base_stride < 0 || p.out_stride < p.N)) return LUTGEMM_EINVAL;
         if (p.out_f16 == p.base_f16 && p.M > 1 && p.out_stride != p.base_stride) return LUTGEMM_EINVAL;
     }
@@ -139,7 +362,37 @@ int check(int count, const lutgemm_adapters *ps)
     return LUTGEMM_OK;
 }
 
-size_t h_bytes(const lutgemm_adapters &p) { return ((size_t)p.M * p.rank * 4 + 15) / 16 * 16; }
+// How a problem is cut, and the bytes of workspace that it takes.
+struct Cut {
+    int slots, k_splits, k_own, n_own;
+    size_t h_bytes, tile_bytes, order_bytes;
+    size_t bytes() const { return h_bytes + tile_bytes + order_bytes; }
+};
+
+size_t round16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+
+Cut cut_of(const lutgemm_adapters &p)
+{
+    Cut c;
+    const bool sorted = p.M > kUnsorted;
+    // tiles: full ones, and one for each kind of rows that is left
+    const int kinds = p.adapters + 1 < p.M ? p.adapters + 1 : p.M;
+    c.slots = sorted ? p.M / kTile + kinds : p.M;
+    const int expected = sorted ? (p.M + kTile - 1) / kTile : p.M;
+    // workgroups enough for the CUs, as long as each wave has a step of its own
+    const int most = (p.K + kWaves * kDepth - 1) / (kWaves * kDepth);
+    int splits = (1024 + expected - 1) / expected;
+    if (splits > most) splits = most;
+    if (splits > 32) splits = 32;
+    const int steps = (p.K + kDepth - 1) / kDepth;
+    c.k_own = (steps + splits - 1) / splits * kDepth;
+    c.k_splits = (p.K + c.k_own - 1) / c.k_own;
+    c.n_own = expected >= 128 ? 4 * kWaves * kColumns : kWaves * kColumns;
+    c.h_bytes = round16((size_t)c.k_splits * p.M * p.rank * 4);
+    c.tile_bytes = sorted ? round16((size_t)c.slots * sizeof(Tile)) : 0;
+    c.order_bytes = sorted ? round16((size_t)p.M * 4) : 0;
+    return c;
+}
 
 }  // namespace
 
@@ -149,7 +402,7 @@ size_t lutgemm_adapters_workspace(int count, const lutgemm_adapters *problems)
 {
     if (check(count, problems) != LUTGEMM_OK) return 0;
     size_t bytes = 0;
-    for (int i = 0; i < count; ++i) bytes += h_bytes(problems[i]);
+    for (int i = 0; i < count; ++i) bytes += cut_of(problems[i]).bytes();
     return bytes;
 }
 
@@ -157,26 +410,51 @@ int lutgemm_adapters_f16(int count, const lutgemm_adapters *problems, void *work
 {
     const int rc = check(count, problems);
     if (rc != LUTGEMM_OK) return rc;
-    if (!workspace || workspace_bytes < lutgemm_adapters_workspace(count, problems)) return LUTGEMM_EINVAL;
-    if (!aligned(workspace, 16)) return LUTGEMM_EALIGN;
+    if (!workspace) return LUTGEMM_EINVAL;
     Args a{};
     a.count = count;
-    char *h = (char *)workspace;
-    int rows = 0, columns = 0;
+    char *at = (char *)workspace;
+    size_t bytes = 0;
+    int slots = 0, splits = 0, chunks = 0, rank = 0;
+    bool sorted = false;
     for (int i = 0; i < count; ++i) {
         const lutgemm_adapters &p = problems[i];
+        const Cut c = cut_of(p);
+        const bool own_order = c.order_bytes > 0;
         a.p[i] = {(const _Float16 *)p.x_f16, (const _Float16 *)p.base_f16, (_Float16 *)p.out_f16, p.ids, (const _Float16 *)p.down_f16,
-                  (const _Float16 *)p.up_f16, p.scale, p.x_stride, p.base_stride, p.out_stride, p.M, p.N, p.K, p.rank, p.adapters, (float *)h};
-        h += h_bytes(p);
-        rows = p.M > rows ? p.M : rows;
-        columns = p.N > columns ? p.N : columns;
+                  (const _Float16 *)p.up_f16, p.scale, p.x_stride, p.base_stride, p.out_stride, p.M, p.N, p.K, p.rank, p.adapters,
+                  c.slots, c.k_splits, c.k_own, c.n_own, (float *)at, own_order ? (Tile *)(at + c.h_bytes) : nullptr,
+                  own_order ? (int32_t *)(at + c.h_bytes + c.tile_bytes) : nullptr};
+        at += c.bytes();
+        bytes += c.bytes();
+        slots = c.slots > slots ? c.slots : slots;
+        splits = c.k_splits > splits ? c.k_splits : splits;
+        const int own_chunks = (p.N + c.n_own - 1) / c.n_own;
+        chunks = own_chunks > chunks ? own_chunks : chunks;
+        rank = p.rank > rank ? p.rank : rank;
+        sorted |= own_order;
     }
+    if (workspace_bytes < bytes) return LUTGEMM_EINVAL;
+    if (!aligned(workspace, 16)) return LUTGEMM_EALIGN;
     const hipStream_t hs = (hipStream_t)stream;
-    hipLaunchKernelGGL(down_kernel, dim3(rows, count), dim3(kThreads), 0, hs, a);
-    const int status = launch_status();
-    if (status != LUTGEMM_OK) return status;
-    hipLaunchKernelGGL(up_kernel, dim3((columns + 4 * kThreads - 1) / (4 * kThreads), rows, count), dim3(kThreads), 0, hs, a);
-    return launch_status();
+    const dim3 threads(kThreads), down_grid(slots, splits, count), up_grid(slots, chunks, count);
+    if (sorted) {
+        hipLaunchKernelGGL(sort_kernel, dim3(count), dim3(1024), 0, hs, a);
+        const int status = launch_status();
+        if (status != LUTGEMM_OK) return status;
+    }
+    auto launch = [&](auto down, auto up) {
+        hipLaunchKernelGGL(down, down_grid, threads, 0, hs, a);
+        const int status = launch_status();
+        if (status != LUTGEMM_OK) return status;
+        hipLaunchKernelGGL(up, up_grid, threads, 0, hs, a);
+        return launch_status();
+    };
+    if (rank <= 16) return launch(down_kernel<1>, up_kernel<1>);
+    if (rank <= 32) return launch(down_kernel<2>, up_kernel<1>);
+    if (rank <= 64) return launch(down_kernel<4>, up_kernel<2>);
+    if (rank <= 128) return launch(down_kernel<8>, up_kernel<4>);
+    return launch(down_kernel<16>, up_kernel<8>);
 }
 
 }  // extern "C"

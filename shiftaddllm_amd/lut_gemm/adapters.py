@@ -25,8 +25,8 @@ class AdapterBank(nn.Module):
         super().__init__()
         if infeatures < 32 or infeatures % 32 or outfeatures < 4 or outfeatures % 4:
             raise ValueError("infeatures must be a multiple of 32, outfeatures a multiple of 4")
-        if not 1 <= rank <= 256 or not 1 <= count <= 65535:
-            raise ValueError("rank must be 1 to 256, count 1 to 65535")
+        if not 1 <= rank <= 256 or not 1 <= count <= native.MAX_ADAPTERS:
+            raise ValueError(f"rank must be 1 to 256, count 1 to {native.MAX_ADAPTERS}")
         self.K, self.N, self.count, self.rank = infeatures, outfeatures, count, -(-rank // 8) * 8
         self.register_buffer("down", torch.zeros((count, self.rank, infeatures), dtype=torch.float16))
         self.register_buffer("up", torch.zeros((count, outfeatures, self.rank), dtype=torch.float16))

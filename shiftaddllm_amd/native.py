@@ -74,6 +74,7 @@ OPTIONS = {"TARGET_BLOCKS": 0, "FIRST_SHARE": 1, "MFMA_MIN_M": 2, "MFMA_BLOCKS":
 CHAIN_MAX_ROWS = 4
 CHAIN_MAX_TAG = 65534
 NOALLOC_MAX_WORDS = 1 << 18
+MAX_ADAPTERS = 8192
 
 
 class RowwiseProblem(ctypes.Structure):
