@@ -52,7 +52,7 @@ struct Problem {
     int n_own;                 // outputs a workgroup takes
     float *h;                  // [k_splits][M][rank]
     Tile *tiles;               // sorted rows: the tiles (a count of 0 behind the last), and
-    int32_t *order;            // the rows
+    int32_t *order, *places;   // the rows, and each one's place among its adapter's
 };
 
 struct Args {
@@ -99,33 +99,52 @@ __device__ int rows_of(const Problem &p, int slot, int (&rows)[kTile], unsigned 
     return min(all - before_slot, kTile);
 }
 
-// Sorts the rows of a problem by adapter (rows without one last) and cuts them into tiles.  One workgroup; the order of an adapter's rows is
-// any, which makes no difference to results.
+// Sorts the rows of a problem by adapter (rows without one in a tile of their own) and cuts them into tiles.  One workgroup; the order of
+// adapters and of an adapter's rows is any, which makes no difference to results.  Bound by its chain of round trips: a row's place among
+// its adapter's is found once and kept.
 __global__ void __launch_bounds__(1024) sort_kernel(const Args args)
 {
-    constexpr int kOwn = (kMaxAdapters + 1 + 1023) / 1024;
+    constexpr int kOwn = (kMaxAdapters + 1 + 1023) / 1024, kRows = 4;
     __shared__ int rows[kMaxAdapters + 1];
     __shared__ int wave_rows[16], wave_tiles[16];
     const Problem &p = args.p[blockIdx.x];
     if (!p.order) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kinds = p.adapters + 1;
     for (int a = tid; a < kinds; a += 1024) rows[a] = 0;
-    __syncthreads();
     auto kind_of = [&](int m) {
-        const int id = adapter_of(p, m);
+        const int id = m < p.M ? adapter_of(p, m) : 0;
         return id < 0 ? p.adapters : id;
     };
-    for (int m = tid; m < p.M; m += 1024) atomicAdd(&rows[kind_of(m)], 1);
+    __syncthreads();
+    for (int m0 = tid; m0 - tid < p.M; m0 += kRows * 1024) {
+        int kind[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) kind[i] = kind_of(m0 + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            // Additions to one address are made one after the other, and the rows of a prompt are beside each other: those of a wave's
+            // first row's kind are added at once.
+            const int m = m0 + 1024 * i, its = __builtin_amdgcn_readfirstlane(kind[i]);
+            const unsigned long long same = __ballot(m < p.M && kind[i] == its);
+            int place = 0;
+            if (lane == 0 && same) place = atomicAdd(&rows[its], __popcll(same));
+            place = __builtin_amdgcn_readfirstlane(place) + __popcll(same & ((1ull << lane) - 1));
+            if (m >= p.M) continue;
+            if (kind[i] != its) place = atomicAdd(&rows[kind[i]], 1);
+            p.places[m] = place;
+        }
+    }
     __syncthreads();
     int own[kOwn], own_rows = 0, own_tiles = 0;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-        const int a = tid * kOwn + i;
+        const int a = tid + 1024 * i;
         own[i] = a < kinds ? rows[a] : 0;
         own_rows += own[i];
         own_tiles += (own[i] + kTile - 1) / kTile;
     }
     int to_rows = own_rows, to_tiles = own_tiles;
+#pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const int r = __shfl_up(to_rows, d), t = __shfl_up(to_tiles, d);
         to_rows += lane >= d ? r : 0;
@@ -137,26 +156,47 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Args args)
     }
     __syncthreads();
     int first = to_rows - own_rows, tile = to_tiles - own_tiles, tiles = 0;
+#pragma unroll
     for (int w = 0; w < 16; ++w) {
         first += w < wave ? wave_rows[w] : 0;
         tile += w < wave ? wave_tiles[w] : 0;
         tiles += wave_tiles[w];
     }
-#pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-        const int a = tid * kOwn + i;
-        if (a >= kinds) break;
-        rows[a] = first;   // (from here on: where the adapter's next row goes)
-        for (int r = 0; r < own[i]; r += kTile) p.tiles[tile++] = {a < p.adapters ? a : -1, first + r, min(own[i] - r, kTile)};
-        first += own[i];
+        const int a = tid + 1024 * i;
+        if (a - tid >= kinds) break;
+        const int mine = a < kinds ? rows[a] : 0;   // (own[i]; still a count)
+        // a kind of many tiles is written by the whole wave, one of few by its thread
+        unsigned long long large = __ballot(mine > 4 * kTile);
+        while (large) {
+            const int l = __ffsll((long long)large) - 1, its_rows = __shfl(mine, l), its_first = __shfl(first, l), its_tile = __shfl(tile, l), its = __shfl(a, l);
+            for (int t = lane; t * kTile < its_rows; t += 64)
+                p.tiles[its_tile + t] = {its < p.adapters ? its : -1, its_first + t * kTile, min(its_rows - t * kTile, kTile)};
+            large &= large - 1;
+        }
+        if (mine <= 4 * kTile)
+            for (int t = 0; t * kTile < mine; ++t) p.tiles[tile + t] = {a < p.adapters ? a : -1, first + t * kTile, min(mine - t * kTile, kTile)};
+        if (a < kinds) rows[a] = first;   // (from here on: where the kind's rows begin)
+        first += mine;
+        tile += (mine + kTile - 1) / kTile;
     }
     for (int t = tiles + tid; t < p.slots; t += 1024) p.tiles[t] = {-1, 0, 0};
     __syncthreads();
-    for (int m = tid; m < p.M; m += 1024) p.order[atomicAdd(&rows[kind_of(m)], 1)] = m;
+    for (int m0 = tid; m0 < p.M; m0 += kRows * 1024) {
+        int kind[kRows], place[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            kind[i] = kind_of(m0 + 1024 * i);
+            place[i] = p.places[min(m0 + 1024 * i, p.M - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (m0 + 1024 * i < p.M) p.order[rows[kind[i]] + place[i]] = m0 + 1024 * i;
+    }
 }
 
-// A part of h for the rows of a tile.  A wave takes 128 inputs at a time, a lane 32 of them side by side (64 bytes of a row of x and of
-// each row of down), eight for each instruction: the inputs are summed over in any order, as long as both operands keep it.
+// A part of h for the rows of a tile.  A wave takes 128 inputs at a time, 32 to an instruction, so that its loads cover 64 bytes of a row
+// side by side.
 template <int NT>   // tiles of 16 ranks, at least as many as there are
 __global__ void __launch_bounds__(kThreads) down_kernel(const Args args)
 {
@@ -176,21 +216,42 @@ __global__ void __launch_bounds__(kThreads) down_kernel(const Args args)
     f32x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = from + wave * kDepth; k0 < to; k0 += kWaves * kDepth) {
-        const int k = k0 + quad * 32;
-        const bool inside = k < p.K;   // (a lane's 32 inputs are there or not, all of them)
-        f16x8 xv[4];
+    // (operands of the next inputs are asked for before these are multiplied; of more than 64 ranks those of x only)
+    constexpr int kAhead = NT <= 4 ? NT : 0;
+    const f16x8 zero = (f16x8)((_Float16)0.0f);
+    f16x8 xv[4], dv[kAhead > 0 ? kAhead : 1][4];
+    auto row_of = [&](int t, int k) { return down + (size_t)min(16 * t + column, p.rank - 1) * p.K + k; };
+    auto fetch = [&](int k0) {
+        const int k = k0 + quad * 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) xv[i] = inside ? *(const f16x8 *)(x + k + 8 * i) : (f16x8)((_Float16)0.0f);
+        for (int i = 0; i < 4; ++i) xv[i] = k0 + 32 * i < p.K ? *(const f16x8 *)(x + k + 32 * i) : zero;
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t)
+            if (t < rank_tiles) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dv[t][i] = k0 + 32 * i < p.K ? *(const f16x8 *)(row_of(t, k) + 32 * i) : zero;
+            }
+    };
+    int k0 = from + wave * kDepth;
+    if (k0 < to) fetch(k0);
+    for (; k0 < to; k0 += kWaves * kDepth) {
+        const int k = k0 + quad * 8;
+        f16x8 xc[4], dc[kAhead > 0 ? kAhead : 1][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            xc[i] = xv[i];
+#pragma unroll
+            for (int t = 0; t < kAhead; ++t) dc[t][i] = dv[t][i];
+        }
+        if (k0 + kWaves * kDepth < to) fetch(k0 + kWaves * kDepth);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if (t < rank_tiles) {
-                const _Float16 *row = down + (size_t)min(16 * t + column, p.rank - 1) * p.K + k;
-                f16x8 dv[4];
+                f16x8 d[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dv[i] = inside ? *(const f16x8 *)(row + 8 * i) : (f16x8)((_Float16)0.0f);
+                for (int i = 0; i < 4; ++i) d[i] = t < kAhead ? dc[t < kAhead ? t : 0][i] : k0 + 32 * i < p.K ? *(const f16x8 *)(row_of(t, k) + 32 * i) : zero;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(dv[i], xv[i], acc[t], 0, 0, 0);
+                for (int i = 0; i < 4; ++i) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d[i], xc[i], acc[t], 0, 0, 0);
             }
         }
     }
@@ -236,23 +297,51 @@ __global__ void __launch_bounds__(kThreads) up_kernel(const Args args)
         }
         return;
     }
+    // What a wave multiplies and adds to is asked for ahead: before h is there, and for the next outputs before these are done.
+    const int m = rows[min(column, count - 1)];
+    const _Float16 *base = p.base + m * p.base_stride;
+    _Float16 *out = p.out + m * p.out_stride;
+    const _Float16 *up = p.up + (size_t)id * p.N * p.rank;
+    typedef _Float16 f16x8_by4 __attribute__((ext_vector_type(8), aligned(8)));   // (base and out are 8-byte aligned)
+    f16x8 ahead[4][RT], added[2];
+    auto fetch = [&](int n0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            // instruction t's row `column` is output (column / 4) * 16 + 4 t + column % 4
+            const _Float16 *row = up + (size_t)min(n0 + column / 4 * 16 + 4 * t + column % 4, p.N - 1) * p.rank;
+#pragma unroll
+            for (int s = 0; s < RT; ++s) {
+                const int r = 32 * s + 8 * quad;
+                ahead[t][s] = r < p.rank ? *(const f16x8 *)(row + r) : (f16x8)((_Float16)0.0f);
+            }
+        }
+        // a lane's 16 outputs, by eights; eight that are not there whole are looked for when they are needed
+        const int n = n0 + 16 * quad;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (n + 8 * h + 8 <= to) added[h] = *(const f16x8_by4 *)(base + n + 8 * h);
+    };
+    int n0 = from + wave * kColumns;
+    if (n0 < to) fetch(n0);
     {   // h of the rows: 16 threads each
         const int row = tid / 16, part = tid % 16;
         const bool live = row < count;
         const float *h = p.h + (size_t)rows[live ? row : 0] * p.rank;
         float v[RT * 2], most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < RT * 2; ++i) {
-            const int r = part + 16 * i;
-            v[i] = 0.0f;
-            if (r < p.rank && live) {
+        for (int i = 0; i < RT * 2; ++i) v[i] = 0.0f;
 #pragma unroll 4
-                for (int s = 0; s < p.k_splits; ++s) v[i] += h[(size_t)s * p.M * p.rank + r];
+        for (int s = 0; s < p.k_splits; ++s) {
+#pragma unroll
+            for (int i = 0; i < RT * 2; ++i) {
+                const int r = part + 16 * i;
+                v[i] += r < p.rank && live ? h[(size_t)s * p.M * p.rank + r] : 0.0f;
             }
-            most = fmaxf(most, fabsf(v[i]));
         }
 #pragma unroll
-        for (int m = 1; m < 16; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+        for (int i = 0; i < RT * 2; ++i) most = fmaxf(most, fabsf(v[i]));
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
         // (a power of two not below the largest, inside what can be inverted; infinite rows stay as they are)
         const int exponent = most > 0.0f && most < INFINITY ? min(max(__builtin_amdgcn_frexp_expf(most), -100), 100) : 0;
 #pragma unroll
@@ -272,38 +361,39 @@ __global__ void __launch_bounds__(kThreads) up_kernel(const Args args)
         lo[t] = *(const f16x8 *)&low[column][32 * t + 8 * quad];
     }
     const float scale = back[column];
-    const int m = rows[min(column, count - 1)];
-    const _Float16 *base = p.base + m * p.base_stride;
-    _Float16 *out = p.out + m * p.out_stride;
-    const _Float16 *up = p.up + (size_t)id * p.N * p.rank;
-    for (int n0 = from + wave * kColumns; n0 < to; n0 += kWaves * kColumns) {
+    for (; n0 < to; n0 += kWaves * kColumns) {
         f32x4 acc[4];
+        f16x8 b[2];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-            // instruction t's row `column` is output (column / 4) * 16 + 4 t + column % 4
-            const int n = min(n0 + column / 4 * 16 + 4 * t + column % 4, p.N - 1);
-            const _Float16 *row = up + (size_t)n * p.rank;
 #pragma unroll
             for (int s = 0; s < RT; ++s) {
-                if (32 * s < p.rank) {
-                    const int r = 32 * s + 8 * quad;
-                    const f16x8 u = r < p.rank ? *(const f16x8 *)(row + r) : (f16x8)((_Float16)0.0f);
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, hi[s], acc[t], 0, 0, 0);
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u, lo[s], acc[t], 0, 0, 0);
-                }
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[t][s], hi[s], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahead[t][s], lo[s], acc[t], 0, 0, 0);
             }
         }
-        if (column >= count) continue;
+        b[0] = added[0];
+        b[1] = added[1];
+        if (n0 + kWaves * kColumns < to) fetch(n0 + kWaves * kColumns);
+        if (column < count) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int n = n0 + 16 * quad + 4 * t;
-            if (n >= to) continue;
-            const f16x4 b = *(const f16x4 *)(base + n);
-            f16x4 o;
+            for (int h = 0; h < 2; ++h) {
+                const int n = n0 + 16 * quad + 8 * h;
+                auto result = [&](int i, _Float16 was) { return (_Float16)fmaf(acc[2 * h + i / 4][i % 4], scale, (float)was); };
+                if (n + 8 <= to) {
+                    f16x8 o;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = (_Float16)fmaf(acc[t][i], scale, (float)b[i]);
-            *(f16x4 *)(out + n) = o;
+                    for (int i = 0; i < 8; ++i) o[i] = result(i, b[h][i]);
+                    *(f16x8_by4 *)(out + n) = o;
+                } else if (n < to) {
+                    const f16x4 was = *(const f16x4 *)(base + n);
+                    f16x4 o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = result(i, was[i]);
+                    *(f16x4 *)(out + n) = o;
+                }
+            }
         }
     }
 }
@@ -387,10 +477,13 @@ Cut cut_of(const lutgemm_adapters &p)
     const int steps = (p.K + kDepth - 1) / kDepth;
     c.k_own = (steps + splits - 1) / splits * kDepth;
     c.k_splits = (p.K + c.k_own - 1) / c.k_own;
-    c.n_own = expected >= 128 ? 4 * kWaves * kColumns : kWaves * kColumns;
+    // (as many workgroups as the CUs hold at once; each finds its rows and their h first.  48 rows 4096 to 11008 of rank 64: 1024 workgroups
+    // 26.0 us, 2048 29.1, 512 26.9)
+    const int chunks = (p.N + kWaves * kColumns - 1) / (kWaves * kColumns), wanted = (1024 + expected - 1) / expected;
+    c.n_own = (chunks + wanted - 1) / wanted * kWaves * kColumns;
     c.h_bytes = round16((size_t)c.k_splits * p.M * p.rank * 4);
     c.tile_bytes = sorted ? round16((size_t)c.slots * sizeof(Tile)) : 0;
-    c.order_bytes = sorted ? round16((size_t)p.M * 4) : 0;
+    c.order_bytes = sorted ? round16((size_t)p.M * 8) : 0;
     return c;
 }
 
@@ -424,7 +517,8 @@ int lutgemm_adapters_f16(int count, const lutgemm_adapters *problems, void *work
         a.p[i] = {(const _Float16 *)p.x_f16, (const _Float16 *)p.base_f16, (_Float16 *)p.out_f16, p.ids, (const _Float16 *)p.down_f16,
                   (const _Float16 *)p.up_f16, p.scale, p.x_stride, p.base_stride, p.out_stride, p.M, p.N, p.K, p.rank, p.adapters,
                   c.slots, c.k_splits, c.k_own, c.n_own, (float *)at, own_order ? (Tile *)(at + c.h_bytes) : nullptr,
-                  own_order ? (int32_t *)(at + c.h_bytes + c.tile_bytes) : nullptr};
+                  own_order ? (int32_t *)(at + c.h_bytes + c.tile_bytes) : nullptr,
+                  own_order ? (int32_t *)(at + c.h_bytes + c.tile_bytes) + p.M : nullptr};
         at += c.bytes();
         bytes += c.bytes();
         slots = c.slots > slots ? c.slots : slots;

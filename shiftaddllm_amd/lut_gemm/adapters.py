@@ -63,7 +63,8 @@ class AdapterBank(nn.Module):
     def forward(self, x, ids, base, out=None):
         """base + scale[id] * up[id] (down[id] x), row by row: x [..., infeatures], base [..., outfeatures] fp16, ids int32, one per row;
         rows whose id is not in 0 .. count - 1 are base's.  `out` may be base itself."""
-        return native.lutgemm.adapters_apply(x, ids, base, out, self.down, self.up, self.scale)
+        b = self._buffers
+        return native.lutgemm.adapters_apply(x, ids, base, out, b["down"], b["up"], b["scale"])
 
     def extra_repr(self):
         return f"in_features={self.K}, out_features={self.N}, rank={self.rank}, count={self.count}"
