@@ -24,6 +24,7 @@
 namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -103,17 +104,20 @@ __device__ __forceinline__ Held quantise(f16x8 x)
     }
     h.low = (_Float16)low;   // (exact: one of the numbers, or +-60000)
     h.scale = (_Float16)(float)(((double)high - (double)low) / 15.0);
-    const double s = (double)(float)h.scale;
     const float inverse = (float)h.scale > 0.0f ? 1.0f / (float)h.scale : 0.0f;
     h.codes = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // The nearest code, exactly: the quotient in fp32 is off by far less than one, what is left over is exact in 64 bits.
-        int c = (int)fminf(rintf((f[i] - low) * inverse), 15.0f);
-        const double rest = ((double)f[i] - (double)low) - c * s;
-        if (2.0 * rest > s || (2.0 * rest == s && (c & 1))) ++c;
-        else if (-2.0 * rest > s || (-2.0 * rest == s && (c & 1))) --c;
-        c = s > 0.0 ? min(max(c, 0), 15) : 0;
+        // The nearest code, exactly: the quotient in fp32 is off by less than 2^-17 (two roundings and the inverse's, of at most 15.01);
+        // where that might decide, what is left over is compared in 64 bits, where it is exact.
+        const float quotient = (f[i] - low) * inverse;
+        int c = (int)fminf(rintf(quotient), 15.0f);
+        if (fabsf(fabsf(quotient - (float)c) - 0.5f) < 0x1p-16f && h.scale > (_Float16)0.0f) {
+            const double s = (double)(float)h.scale, rest = ((double)f[i] - (double)low) - c * s;
+            if (2.0 * rest > s || (2.0 * rest == s && (c & 1))) ++c;
+            else if (-2.0 * rest > s || (-2.0 * rest == s && (c & 1))) --c;
+            c = min(max(c, 0), 15);
+        }
         h.codes |= (uint32_t)c << (4 * i);
         h.value[i] = __builtin_fmaf16((_Float16)(float)c, h.scale, h.low);
     }
@@ -229,61 +233,136 @@ __device__ __forceinline__ int blocks_per_split(const Args &a, int blocks, int l
     return max((blocks + a.splits - 1) / a.splits, least);
 }
 
-// A wave takes 16 RT query rows of a (sequence, kv head) pair.  APART: the waves of a workgroup take different rows and all of
-// the workgroup's blocks (long prompts); otherwise they take the same rows, and the blocks in turn.
-template <int G, int RT, bool APART>
+// The queries of 16 RT rows from row0 on, as the matrix instruction's B operand, and the last position that each row attends to.  Rows
+// behind the last live one repeat it.
+template <int G, int RT>
+__device__ __forceinline__ void load_queries(const Args &a, int b, int kvh, int start, int row0, int live_rows, f16x8 (&q)[RT][G], int (&limit)[RT])
+{
+    const int lane = threadIdx.x & 63, column = lane & 15, quad = lane >> 4;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row0 + 16 * rt + column, max(live_rows, 1) - 1), token = row / a.rep;
+        limit[rt] = start + token;
+        const _Float16 *head = a.q + b * a.q_stride[0] + token * a.q_stride[1] + (size_t)(kvh * a.rep + row % a.rep) * (32 * G);
+        const size_t angle = (size_t)(start + token) * (32 * G);
+#pragma unroll
+        for (int t = 0; t < G; ++t) q[rt][t] = rotated(head, a.cos_t + angle, a.sin_t + angle, 32 * t + 8 * quad, 32 * G);
+    }
+}
+
+// Of one row a lane: the reference (a score), the sum of weights 2^(factor * (score - reference)), and the weighted values.
+template <int G>
+struct RowState {
+    float reference, sum;
+    f32x4 acc[2 * G];
+    __device__ __forceinline__ void clear()
+    {
+        reference = -1e30f;
+        sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // The weights of a block's scores (half h of the block: positions j0 + 16 h + 4 quad + i); `edge`: some may lie behind `limit`.
+    __device__ __forceinline__ f16x8 weights(const f32x4 (&score)[2], float factor, bool edge, int j0, int limit)
+    {
+        const int quad = (threadIdx.x & 63) >> 4;
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = score[e / 4][e % 4];
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = j0 + 16 * (e / 4) + 4 * quad + e % 4 <= limit ? s[e] : -INFINITY;
+        }
+        float most = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        if (__any((most - reference) * factor > kSlack)) {
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float raised = fmaxf(reference, most), keep = __builtin_amdgcn_exp2f((reference - raised) * factor);
+            reference = raised;
+            sum *= keep;
+#pragma unroll
+            for (int t = 0; t < 2 * G; ++t) acc[t] *= keep;
+        }
+        const float off = -reference * factor;
+        f16x8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[e], factor, off));
+            sum += p;
+            w[e] = (_Float16)p;
+        }
+        return w;
+    }
+    __device__ __forceinline__ void finish()
+    {
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+    }
+};
+
+// Scales and minima of values at positions behind `last` become zero: whatever is there has no influence.
+__device__ __forceinline__ uint32_t live_mask(int i, int j0, int last)
+{
+    const int quad = (threadIdx.x & 63) >> 4, p = j0 + 16 * (i / 2) + 4 * quad + 2 * (i % 2);
+    return (p <= last ? 0xffffu : 0u) | (p + 1 <= last ? 0xffff0000u : 0u);
+}
+
+// Four numbers of a row at dimension d: value / total into out, or, where workgroups share positions, value with the row's reference
+// (in powers of two) and total beside it.
+template <int HD>
+__device__ __forceinline__ void store_row(const Args &a, int b, int kvh, int pair, int split, int unit, int unit_rows, int row, int live_rows, int d,
+                                          f32x4 value, float reference, float total)
+{
+    if (row >= a.tokens * a.rep) return;
+    if (a.splits > 1) {
+        const size_t at = (((size_t)split * a.pairs + pair) * a.units + unit) * unit_rows + (row - unit * unit_rows);
+        *(f32x4 *)(a.partial + at * HD + d) = value;
+        if (d == 0) a.stats[at] = make_float2(reference, total);
+        return;
+    }
+    const int token = row / a.rep;
+    const float inverse = row < live_rows ? 1.0f / total : 0.0f;
+    if (row >= live_rows) value = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const f16x4 o = {(_Float16)(value[0] * inverse), (_Float16)(value[1] * inverse), (_Float16)(value[2] * inverse), (_Float16)(value[3] * inverse)};
+    *(f16x4 *)(a.out + (((size_t)b * a.tokens + token) * a.heads + kvh * a.rep + row % a.rep) * HD + d) = o;
+}
+
+__device__ __forceinline__ f16x8 vector_of(const uint32_t (&w)[4]) { return __builtin_bit_cast(f16x8, (u32x4){w[0], w[1], w[2], w[3]}); }
+
+// Few query rows: the waves of a workgroup take the same 16 RT rows, and the blocks in turn, each block from memory to registers.
+// Bound by the stream of the cache: a wave holds a block at a time, the next one's keys are asked for when its scores are formed, its
+// values once they are folded in.
+template <int G, int RT>
 __global__ void __launch_bounds__(kThreads) attention_kernel(const Args a)
 {
     constexpr int HD = 32 * G, ROWS = 16 * RT;
     constexpr int kTilesAtOnce = RT == 1 ? 8 : 4;   // of 16 dimensions, joined at a time
     constexpr int kPadded = 16 * kTilesAtOnce + 4;
-    __shared__ float joined[APART ? 1 : kWaves][APART ? 1 : ROWS][APART ? 1 : kPadded];
+    __shared__ float joined[kWaves][ROWS][kPadded];
     __shared__ float2 wave_stats[kWaves][ROWS];
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int column = lane & 15, quad = lane >> 4;
     const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
-    const int split = rest % a.splits, tile = a.tiles - 1 - rest / a.splits;   // (the longest rows of a prompt first)
+    const int split = rest % a.splits, tile = a.tiles - 1 - rest / a.splits;
     const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
     int start;
     const int n = live_tokens(a, b, start);
-    const int unit = APART ? tile * kWaves + wave : tile;
-    const int row0 = unit * ROWS, all_rows = a.tokens * a.rep, live_rows = n * a.rep;
-
-    // the blocks of this workgroup
-    const int tile_rows = APART ? kWaves * ROWS : ROWS;
-    const int tile_last = min((tile + 1) * tile_rows, live_rows) - 1;          // its last row that is no padding
-    const int tile_blocks = tile_last >= tile * tile_rows ? (start + tile_last / a.rep) / kBlock + 1 : 0;
-    const int per = blocks_per_split(a, tile_blocks, APART ? 4 : kWaves);
-    const int begin = split * per;
-    int end = min(begin + per, tile_blocks);
-    const int last = min(row0 + ROWS, live_rows) - 1;                          // of this wave
+    const int row0 = tile * ROWS, live_rows = n * a.rep;
+    const int last = min(row0 + ROWS, live_rows) - 1;                          // its last row that is no padding
     const int limit_high = last >= row0 ? start + last / a.rep : -1, limit_low = start + row0 / a.rep;
-    if (APART) end = min(end, (limit_high + kBlock) / kBlock);
-    if (!APART && a.splits > 1 && begin >= end) return;                        // (nobody reads its part)
+    const int blocks = (limit_high + kBlock) / kBlock;
+    const int per = blocks_per_split(a, blocks, kWaves);
+    const int begin = split * per, end = min(begin + per, blocks);
+    if (a.splits > 1 && begin >= end) return;                                  // (nobody reads its part)
 
     f16x8 q[RT][G];
     int limit[RT];
+    load_queries<G, RT>(a, b, kvh, start, row0, live_rows, q, limit);
+    RowState<G> state[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = min(row0 + 16 * rt + column, max(live_rows, 1) - 1), token = row / a.rep;
-        limit[rt] = start + token;
-        const _Float16 *head = a.q + b * a.q_stride[0] + token * a.q_stride[1] + (size_t)(kvh * a.rep + row % a.rep) * HD;
-        const size_t angle = (size_t)(start + token) * HD;
-#pragma unroll
-        for (int t = 0; t < G; ++t) q[rt][t] = rotated(head, a.cos_t + angle, a.sin_t + angle, 32 * t + 8 * quad, HD);
-    }
-
-    f32x4 acc[RT][2 * G];
-    float reference[RT], sum[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        reference[rt] = -1e30f;
-        sum[rt] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 2 * G; ++t) acc[rt][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const float to_log2 = 1.4426950408889634f / sqrtf((float)HD);
+    for (int rt = 0; rt < RT; ++rt) state[rt].clear();
+    const float factor = 1.4426950408889634f / sqrtf((float)HD);
     const uint8_t *cache = a.cache + (size_t)pair * a.blocks * (size_t)(1280 * G);
 
     uint32_t k_codes[2][G], k_scales[2][G], v_codes[2 * G], v_scales[2 * G][4];
@@ -301,14 +380,13 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Args a)
 #pragma unroll
         for (int t = 0; t < 2 * G; ++t) load_words(v_scales[t], base + 512 * G + t * 64 + quad * 16);
     };
-    const int step = APART ? 1 : kWaves;
-    int block = begin + (APART ? 0 : wave);
+    int block = begin + wave;
     if (block < end) {
         fetch_keys(block);
         fetch_values(block);
     }
-    for (; block < end; block += step) {
-        const int next = block + step < end ? block + step : block;
+    for (; block < end; block += kWaves) {
+        const int next = block + kWaves < end ? block + kWaves : block;
         f32x4 score[RT][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -329,164 +407,232 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Args a)
         const bool edge = j0 + kBlock - 1 > limit_low;
         f16x8 weight[RT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float s[8], most = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = score[rt][e / 4][e % 4] * to_log2;
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] = j0 + 16 * (e / 4) + 4 * quad + e % 4 <= limit[rt] ? s[e] : -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, s[e]);
-            if (__any(most > reference[rt] + kSlack)) {
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const float raised = fmaxf(reference[rt], most), keep = __builtin_amdgcn_exp2f(reference[rt] - raised);
-                reference[rt] = raised;
-                sum[rt] *= keep;
-#pragma unroll
-                for (int t = 0; t < 2 * G; ++t) acc[rt][t] *= keep;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float p = __builtin_amdgcn_exp2f(s[e] - reference[rt]);
-                sum[rt] += p;
-                weight[rt][e] = (_Float16)p;
-            }
-        }
-        if (j0 + kBlock - 1 > limit_high) {   // positions that no row attends to: whatever is there, times zero
-            uint32_t mask[4];
+        for (int rt = 0; rt < RT; ++rt) weight[rt] = state[rt].weights(score[rt], factor, edge, j0, limit[rt]);
+        if (j0 + kBlock - 1 > limit_high) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int p = j0 + 16 * (i / 2) + 4 * quad + 2 * (i % 2);
-                mask[i] = (p <= limit_high ? 0xffffu : 0u) | (p + 1 <= limit_high ? 0xffff0000u : 0u);
+                const uint32_t mask = live_mask(i, j0, limit_high);
+#pragma unroll
+                for (int t = 0; t < 2 * G; ++t) v_scales[t][i] &= mask;
             }
-#pragma unroll
-            for (int t = 0; t < 2 * G; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v_scales[t][i] &= mask[i];
         }
 #pragma unroll
         for (int t = 0; t < 2 * G; ++t) {
-            const f16x8 scale = __builtin_bit_cast(f16x8, (u32x4){v_scales[t & ~1][0], v_scales[t & ~1][1], v_scales[t & ~1][2], v_scales[t & ~1][3]});
-            const f16x8 low = __builtin_bit_cast(f16x8, (u32x4){v_scales[t | 1][0], v_scales[t | 1][1], v_scales[t | 1][2], v_scales[t | 1][3]});
-            const f16x8 value = __builtin_elementwise_fma(codes_of(v_codes[t]), scale, low);
+            const f16x8 value = __builtin_elementwise_fma(codes_of(v_codes[t]), vector_of(v_scales[t & ~1]), vector_of(v_scales[t | 1]));
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], acc[rt][t], 0, 0, 0);
+            for (int rt = 0; rt < RT; ++rt) state[rt].acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], state[rt].acc[t], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         fetch_values(next);
         __builtin_amdgcn_sched_barrier(0);
     }
+
+    // ---- the waves' results joined ------------------------------------------------------------------------------------------
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        sum[rt] += __shfl_xor(sum[rt], 16);
-        sum[rt] += __shfl_xor(sum[rt], 32);
+        state[rt].finish();
+        state[rt].reference *= factor;   // (in powers of two from here on)
+        if (quad == 0) wave_stats[wave][16 * rt + column] = make_float2(state[rt].reference, state[rt].sum);
     }
-
-    // ---- the rows' results: out, or this split's part -----------------------------------------------------------------------
-    // Four numbers of a row at dimension d: `value` / total, or value with the row's reference and total beside it.
-    auto store = [&](int row, int d, f32x4 value, float reference_, float total) {
-        if (row >= all_rows) return;
-        if (a.splits > 1) {
-            const size_t at = (((size_t)split * a.pairs + pair) * a.units + unit) * ROWS + (row - row0);
-            *(f32x4 *)(a.partial + at * HD + d) = value;
-            if (d == 0) a.stats[at] = make_float2(reference_, total);
-            return;
-        }
-        const int token = row / a.rep;
-        const float inverse = row < live_rows ? 1.0f / total : 0.0f;
-        if (row >= live_rows) value = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-        const f16x4 o = {(_Float16)(value[0] * inverse), (_Float16)(value[1] * inverse), (_Float16)(value[2] * inverse), (_Float16)(value[3] * inverse)};
-        *(f16x4 *)(a.out + (((size_t)b * a.tokens + token) * a.heads + kvh * a.rep + row % a.rep) * HD + d) = o;
-    };
-    if constexpr (APART) {
-        if (unit >= a.units) return;
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float most = wave_stats[0][16 * rt + column].x;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) most = fmaxf(most, wave_stats[w][16 * rt + column].x);
+        const float keep = __builtin_amdgcn_exp2f(state[rt].reference - most);
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t) state[rt].acc[t] *= keep;
+    }
+#pragma unroll
+    for (int t0 = 0; t0 < 2 * G; t0 += kTilesAtOnce) {
+        if (t0 > 0) __syncthreads();
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int t = 0; t < 2 * G; ++t) store(row0 + 16 * rt + column, 16 * t + 4 * quad, acc[rt][t], reference[rt], sum[rt]);
-    } else {
-        if (quad == 0)
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) wave_stats[wave][16 * rt + column] = make_float2(reference[rt], sum[rt]);
+            for (int t = t0; t < t0 + kTilesAtOnce && t < 2 * G; ++t)
+                *(f32x4 *)&joined[wave][16 * rt + column][16 * (t - t0) + 4 * quad] = state[rt].acc[t];
         __syncthreads();
+        const int fours = 4 * min(kTilesAtOnce, 2 * G - t0);
+        for (int u = tid; u < ROWS * fours; u += kThreads) {
+            const int row = u / fours, d = u % fours * 4;
+            f32x4 value = *(const f32x4 *)&joined[0][row][d];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float most = -1e30f;
+            for (int w = 1; w < kWaves; ++w) value += *(const f32x4 *)&joined[w][row][d];
+            float most = wave_stats[0][row].x, total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) most = fmaxf(most, wave_stats[w][16 * rt + column].x);
-            const float keep = __builtin_amdgcn_exp2f(reference[rt] - most);
+            for (int w = 1; w < kWaves; ++w) most = fmaxf(most, wave_stats[w][row].x);
 #pragma unroll
-            for (int t = 0; t < 2 * G; ++t) acc[rt][t] *= keep;
-        }
-#pragma unroll
-        for (int t0 = 0; t0 < 2 * G; t0 += kTilesAtOnce) {
-            if (t0 > 0) __syncthreads();
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int t = t0; t < t0 + kTilesAtOnce && t < 2 * G; ++t)
-                    *(f32x4 *)&joined[wave][16 * rt + column][16 * (t - t0) + 4 * quad] = acc[rt][t];
-            __syncthreads();
-            const int fours = 4 * min(kTilesAtOnce, 2 * G - t0);
-            for (int u = tid; u < ROWS * fours; u += kThreads) {
-                const int row = u / fours, d = u % fours * 4;
-                f32x4 value = *(const f32x4 *)&joined[0][row][d];
-#pragma unroll
-                for (int w = 1; w < kWaves; ++w) value += *(const f32x4 *)&joined[w][row][d];
-                float most = -1e30f, total = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) most = fmaxf(most, wave_stats[w][row].x);
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) total += wave_stats[w][row].y * __builtin_amdgcn_exp2f(wave_stats[w][row].x - most);
-                store(row0 + row, 16 * t0 + d, value, most, total);
-            }
+            for (int w = 0; w < kWaves; ++w) total += wave_stats[w][row].y * __builtin_amdgcn_exp2f(wave_stats[w][row].x - most);
+            store_row<HD>(a, b, kvh, pair, split, tile, ROWS, row0 + row, live_rows, 16 * t0 + d, value, most, total);
         }
     }
 }
 
-// Joins the parts of a row: sum over splits of 2^(reference - largest reference) * part, in the order of the splits.
-// One thread per four dimensions of a row.
-template <int G>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Args a, int rows_per_unit, int units_per_tile)
+// Many query rows (prompts): the waves of a workgroup take 32 rows each, side by side, and all of its blocks together.  A block's keys and
+// values are formed once for all waves, by pieces, and handed over through LDS as the matrix instructions' operands: a wave that forms them for
+// itself does nothing else for most of its time (two prompts of 2048 tokens, 32 heads on 8: 197 us, vector unit 62 % busy, matrix unit 15 %).
+// Two buffers, one barrier a block: while a block is multiplied, the next one is formed and the one behind it asked for.
+template <int G, int W>
+__global__ void __launch_bounds__(64 * W) prompt_kernel(const Args a)
 {
-    constexpr int HD = 32 * G;
-    const int all_rows = a.tokens * a.rep;
-    const long u = (long)blockIdx.x * kThreads + threadIdx.x;
-    const int d = (int)(u % (HD / 4)) * 4;
-    const long at_row = u / (HD / 4);
-    const int pair = (int)(at_row / all_rows), row = (int)(at_row % all_rows);
-    if (pair >= a.pairs) return;
+    constexpr int HD = 32 * G, RT = 2, ROWS = 16 * RT;
+    constexpr int kPieces = (2 * G + W - 1) / W;   // of 2 G operands of keys and as many of values, a wave's
+    __shared__ f16x8 keys[2][2 * G][64], values[2][2 * G][64];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, quad = lane >> 4;
+    const int pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs;
+    const int split = rest % a.splits, tile = a.tiles - 1 - rest / a.splits;   // (the longest rows first)
+    const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
+    int start;
+    const int n = live_tokens(a, b, start);
+    const int unit = tile * W + wave, row0 = unit * ROWS, live_rows = n * a.rep;
+
+    const int tile_last = min((tile + 1) * W * ROWS, live_rows) - 1;
+    const int tile_high = tile_last >= tile * W * ROWS ? start + tile_last / a.rep : -1, blocks = (tile_high + kBlock) / kBlock;
+    const int per = blocks_per_split(a, blocks, 4);
+    const int begin = split * per, end = min(begin + per, blocks);
+    if (a.splits > 1 && begin >= end) return;
+    const int last = min(row0 + ROWS, live_rows) - 1;
+    const int limit_high = last >= row0 ? start + last / a.rep : -1, limit_low = start + row0 / a.rep;
+    const int own_end = min(end, (limit_high + kBlock) / kBlock);              // (the rest lies behind this wave's rows)
+
+    const uint8_t *cache = a.cache + (size_t)pair * a.blocks * (size_t)(1280 * G);
+    uint32_t k_code[kPieces], k_scale[kPieces], v_code[kPieces], v_scale[kPieces][2][4];
+    auto fetch = [&](int block) {
+        const uint8_t *base = cache + (size_t)block * (1280 * G);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int f = wave + i * W, position = 16 * (f / G) + column;
+            if (2 * G % W != 0 && f >= 2 * G) continue;
+            k_code[i] = *(const uint32_t *)(base + ((position * 4 + quad) * G + f % G) * 4);
+            k_scale[i] = *(const uint32_t *)(base + 512 * G + (position * G + f % G) * 4);
+            v_code[i] = *(const uint32_t *)(base + 640 * G + ((quad * 16 + column) * 2 * G + f) * 4);
+            load_words(v_scale[i][0], base + 1152 * G + (f & ~1) * 64 + quad * 16);
+            load_words(v_scale[i][1], base + 1152 * G + (f | 1) * 64 + quad * 16);
+        }
+    };
+    auto form = [&](int block, int buffer) {
+        const bool beyond = (block + 1) * kBlock - 1 > tile_high;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int f = wave + i * W;
+            if (2 * G % W != 0 && f >= 2 * G) continue;
+            const f16x2 sm = __builtin_bit_cast(f16x2, k_scale[i]);
+            keys[buffer][f][lane] = __builtin_elementwise_fma(codes_of(k_code[i]), (f16x8)(sm.x), (f16x8)(sm.y));
+            if (beyond) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t mask = live_mask(j, block * kBlock, tile_high);
+                    v_scale[i][0][j] &= mask;
+                    v_scale[i][1][j] &= mask;
+                }
+            }
+            values[buffer][f][lane] = __builtin_elementwise_fma(codes_of(v_code[i]), vector_of(v_scale[i][0]), vector_of(v_scale[i][1]));
+        }
+    };
+    if (begin < end) fetch(begin);
+    f16x8 q[RT][G];
+    int limit[RT];
+    load_queries<G, RT>(a, b, kvh, start, row0, live_rows, q, limit);
+    RowState<G> state[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) state[rt].clear();
+    const float factor = 1.4426950408889634f / sqrtf((float)HD);
+    if (begin < end) {
+        form(begin, 0);
+        if (begin + 1 < end) fetch(begin + 1);
+    }
+    for (int block = begin; block < end; ++block) {
+        const int buffer = (block - begin) & 1;
+        __syncthreads();   // this block is formed, and the other buffer read
+        if (block + 1 < end) {
+            form(block + 1, buffer ^ 1);
+            if (block + 2 < end) fetch(block + 2);
+        }
+        if (block >= own_end) continue;
+        f32x4 score[RT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) score[rt][h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int t = 0; t < G; ++t) {
+                const f16x8 key = keys[buffer][h * G + t][lane];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) score[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[rt][t], score[rt][h], 0, 0, 0);
+            }
+        }
+        const int j0 = block * kBlock;
+        const bool edge = j0 + kBlock - 1 > limit_low;
+        f16x8 weight[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) weight[rt] = state[rt].weights(score[rt], factor, edge, j0, limit[rt]);
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t) {
+            const f16x8 value = values[buffer][t][lane];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) state[rt].acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], state[rt].acc[t], 0, 0, 0);
+        }
+    }
+    if (unit >= a.units) return;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        state[rt].finish();
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t)
+            store_row<HD>(a, b, kvh, pair, split, unit, ROWS, row0 + 16 * rt + column, live_rows, 16 * t + 4 * quad, state[rt].acc[t], state[rt].reference * factor, state[rt].sum);
+    }
+}
+
+// Joins the parts of a row: the sum over splits of 2^(reference - largest reference) * part.  One workgroup per row; the splits' weights are formed
+// by a lane each, and groups of HD / 4 threads take the splits in turn (one thread for all of a row's splits: 64 splits of 128 rows 43 us).
+constexpr int kMostSplits = 64;
+
+template <int G>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Args a, int unit_rows, int tile_rows, int least)
+{
+    constexpr int HD = 32 * G, kGroups = kThreads / (HD / 4);
+    __shared__ float weight[kMostSplits];
+    __shared__ f32x4 part[kGroups][HD / 4];
+    const int tid = threadIdx.x, pair = blockIdx.x % a.pairs, row = blockIdx.x / a.pairs;
     const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
     int start;
     const int n = live_tokens(a, b, start), live_rows = n * a.rep;
-    const int unit = row / rows_per_unit, tile = unit / units_per_tile, tile_rows = units_per_tile * rows_per_unit;
-    f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
-    float total = 1.0f;
-    if (row < live_rows) {
-        const int tile_last = min((tile + 1) * tile_rows, live_rows) - 1;
-        const int tile_blocks = (start + tile_last / a.rep) / kBlock + 1;
-        const int per = blocks_per_split(a, tile_blocks, units_per_tile > 1 ? 4 : kWaves);
-        const int parts = (tile_blocks + per - 1) / per;
-        const size_t stride = (size_t)a.pairs * a.units * rows_per_unit;
-        const size_t at = ((size_t)pair * a.units + unit) * rows_per_unit + row % rows_per_unit;
-        float most = -1e30f;
-        for (int s = 0; s < parts; ++s) most = fmaxf(most, a.stats[s * stride + at].x);
-        total = 0.0f;
-        for (int s = 0; s < parts; ++s) {
-            const float2 st = a.stats[s * stride + at];
-            const float keep = __builtin_amdgcn_exp2f(st.x - most);
-            total += st.y * keep;
-            value += *(const f32x4 *)(a.partial + (s * stride + at) * HD + d) * keep;
-        }
+    f16x4 *out = (f16x4 *)(a.out + (((size_t)b * a.tokens + row / a.rep) * a.heads + kvh * a.rep + row % a.rep) * HD);
+    if (row >= live_rows) {
+        if (tid < HD / 4) out[tid] = (f16x4)((_Float16)0.0f);
+        return;
     }
+    const int unit = row / unit_rows, tile = row / tile_rows, tile_last = min((tile + 1) * tile_rows, live_rows) - 1;
+    const int blocks = (start + tile_last / a.rep) / kBlock + 1, per = blocks_per_split(a, blocks, least), parts = (blocks + per - 1) / per;
+    const size_t stride = (size_t)a.pairs * a.units * unit_rows, at = ((size_t)pair * a.units + unit) * unit_rows + row % unit_rows;
+    const int lane = tid & 63;
+    float2 st = make_float2(-INFINITY, 0.0f);
+    if (lane < parts) st = a.stats[lane * stride + at];
+    float most = st.x;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+    const float keep = lane < parts ? __builtin_amdgcn_exp2f(st.x - most) : 0.0f;
+    float total = st.y * keep;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) total += __shfl_xor(total, m);
+    if (tid < kMostSplits) weight[tid] = keep;
+    __syncthreads();
+    const int group = tid / (HD / 4), d = tid % (HD / 4);
+    if (group < kGroups) {
+        f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int s = group; s < parts; s += kGroups) value += *(const f32x4 *)(a.partial + (s * stride + at) * HD + 4 * d) * weight[s];
+        part[group][d] = value;
+    }
+    __syncthreads();
+    if (tid >= HD / 4) return;
+    f32x4 value = part[0][tid];
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) value += part[g][tid];
     const float inverse = 1.0f / total;
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    const f16x4 o = {(_Float16)(value[0] * inverse), (_Float16)(value[1] * inverse), (_Float16)(value[2] * inverse), (_Float16)(value[3] * inverse)};
-    *(f16x4 *)(a.out + (((size_t)b * a.tokens + row / a.rep) * a.heads + kvh * a.rep + row % a.rep) * HD + d) = o;
+    out[tid] = (f16x4){(_Float16)(value[0] * inverse), (_Float16)(value[1] * inverse), (_Float16)(value[2] * inverse), (_Float16)(value[3] * inverse)};
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
@@ -516,17 +662,18 @@ int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int 
     const long rows = (long)tokens * (heads / kv_heads), pairs = (long)batch * kv_heads;
     const int blocks = (max_positions + kBlock - 1) / kBlock;
     p->fused = 0;
-    p->threads = kThreads;
     p->rows_per_wave = rows > 16 ? 32 : 16;
     p->rows_apart = rows >= 4 * 32;
+    const int waves = p->rows_apart && rows < 8 * 32 ? 4 : p->rows_apart ? 8 : kWaves;
+    p->threads = 64 * waves;
     s->units = (int)((rows + p->rows_per_wave - 1) / p->rows_per_wave);
-    s->tiles = p->rows_apart ? (s->units + kWaves - 1) / kWaves : s->units;
+    s->tiles = p->rows_apart ? (s->units + waves - 1) / waves : s->units;
     const long alone = pairs * s->tiles;
     long splits = 1;
-    if (alone < 1024) splits = (1024 + alone - 1) / alone;
-    const long most = blocks / (p->rows_apart ? 32 : 32);   // each split has some blocks to itself
+    if (alone * waves < 4096) splits = (4096 + alone * waves - 1) / (alone * waves);
+    const long most = blocks / 32;   // each split has some blocks to itself
     if (splits > most) splits = most;
-    if (splits > 64) splits = 64;
+    if (splits > kMostSplits) splits = kMostSplits;
     if (splits < 1) splits = 1;
     p->splits = (int)splits;
     p->row_tiles = s->tiles;
@@ -536,7 +683,7 @@ int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int 
     const size_t part_rows = (size_t)splits * pairs * s->units * p->rows_per_wave;
     s->partial_floats = splits > 1 ? part_rows * head_dim : 0;
     s->workspace = splits > 1 ? part_rows * (head_dim * 4 + 8) : 0;
-    if ((size_t)pairs * tokens * (heads / kv_heads) * (head_dim / 4) / kThreads > 0x7ffffff0u) return LUTGEMM_EINVAL;
+    if (splits > 1 && pairs * rows > 0x7fffffffl) return LUTGEMM_EINVAL;
     return LUTGEMM_OK;
 }
 
@@ -622,15 +769,16 @@ int lutgemm_q4_attention_f16(const lutgemm_q4_attention *c, void *workspace, siz
         hipLaunchKernelGGL(append_kernel<G>, dim3((unsigned)(parts * a.pairs)), dim3(kThreads), 0, hs, a);
         int status = launch_status();
         if (status != LUTGEMM_OK) return status;
-        const dim3 grid((unsigned)plan.workgroups);
-        if (plan.rows_apart) hipLaunchKernelGGL((attention_kernel<G, 2, true>), grid, dim3(kThreads), 0, hs, a);
-        else if (plan.rows_per_wave == 32) hipLaunchKernelGGL((attention_kernel<G, 2, false>), grid, dim3(kThreads), 0, hs, a);
-        else hipLaunchKernelGGL((attention_kernel<G, 1, false>), grid, dim3(kThreads), 0, hs, a);
+        const dim3 grid((unsigned)plan.workgroups), threads((unsigned)plan.threads);
+        if (plan.rows_apart && plan.threads == 512) hipLaunchKernelGGL((prompt_kernel<G, 8>), grid, threads, 0, hs, a);
+        else if (plan.rows_apart) hipLaunchKernelGGL((prompt_kernel<G, 4>), grid, threads, 0, hs, a);
+        else if (plan.rows_per_wave == 32) hipLaunchKernelGGL((attention_kernel<G, 2>), grid, threads, 0, hs, a);
+        else hipLaunchKernelGGL((attention_kernel<G, 1>), grid, threads, 0, hs, a);
         status = launch_status();
         if (status != LUTGEMM_OK || a.splits == 1) return status;
-        const size_t threads = (size_t)a.pairs * a.tokens * a.rep * (8 * G);
-        hipLaunchKernelGGL(join_kernel<G>, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, hs, a, plan.rows_per_wave,
-                           plan.rows_apart ? kWaves : 1);
+        const int tile_rows = plan.rows_apart ? plan.rows_per_wave * (plan.threads / 64) : plan.rows_per_wave;
+        hipLaunchKernelGGL(join_kernel<G>, dim3((unsigned)((size_t)a.pairs * a.tokens * a.rep)), dim3(kThreads), 0, hs, a, plan.rows_per_wave, tile_rows,
+                           plan.rows_apart ? 4 : kWaves);
         return launch_status();
     };
     switch (c->head_dim / 32) {
