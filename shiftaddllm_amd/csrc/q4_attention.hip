@@ -44,6 +44,7 @@ struct Args {
     int64_t q_stride[2], k_stride[2], v_stride[2];
     int tokens, heads, kv_heads, rep, max_positions, blocks;   // blocks: of a (sequence, kv head) pair in the cache
     int pairs, units, tiles, splits;                           // units: tiles of a wave's rows; tiles: of a workgroup's
+    int fused;                                                 // the attention launch appends
     float *partial;                                            // [split][pair][unit][rows][head_dim], then ...
     float2 *stats;                                             // ... (reference, sum) [split][pair][unit][rows]
 };
@@ -133,51 +134,50 @@ __device__ __forceinline__ uint32_t word_of(uint32_t codes)
     return w;
 }
 
-// One workgroup per block of the cache that new tokens of a (sequence, kv head) pair fall into: it alone writes the block, so that
-// words that hold other positions too can be read, changed and written.  Lanes 4 i .. 4 i + 3 take a group of 32 numbers.
-template <int G>
-__global__ void __launch_bounds__(kThreads) append_kernel(const Args a)
+// Rows of the held values of tokens first .. past - 1 that are passed over: zeros.
+template <int HD>
+__device__ __forceinline__ void clear_held(const Args &a, int b, int kvh, int n, int first, int past)
 {
-    constexpr int HD = 32 * G;
-    __shared__ uint8_t code[kBlock][HD + 4];   // of the values, by position
-    const int tid = threadIdx.x;
-    const int pair = blockIdx.x % a.pairs, part = blockIdx.x / a.pairs;
-    const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
-    int start;
-    const int n = live_tokens(a, b, start);
-    const size_t held_row = (size_t)a.kv_heads * HD;
-    if (a.k_held || a.v_held) {   // rows of tokens that are passed over
-        for (int u = tid; u < kBlock * (HD / 8); u += kThreads) {
-            const int token = part * kBlock + u / (HD / 8);
-            if (token < n || token >= a.tokens) continue;
-            const size_t at = ((size_t)b * a.tokens + token) * held_row + (size_t)kvh * HD + u % (HD / 8) * 8;
-            if (a.k_held) *(u32x4 *)(a.k_held + at) = (u32x4){0, 0, 0, 0};
-            if (a.v_held) *(u32x4 *)(a.v_held + at) = (u32x4){0, 0, 0, 0};
-        }
+    if (!a.k_held && !a.v_held) return;
+    for (int u = threadIdx.x; u < (past - first) * (HD / 8); u += kThreads) {
+        const int token = first + u / (HD / 8);
+        if (token < n) continue;
+        const size_t at = (((size_t)b * a.tokens + token) * a.kv_heads + kvh) * HD + u % (HD / 8) * 8;
+        if (a.k_held) *(u32x4 *)(a.k_held + at) = (u32x4){0, 0, 0, 0};
+        if (a.v_held) *(u32x4 *)(a.v_held + at) = (u32x4){0, 0, 0, 0};
     }
-    const int block = start / kBlock + part;
+}
+
+// The new tokens of a (sequence, kv head) pair whose positions lie in a block of the cache, by a workgroup of kThreads that alone writes the
+// block, so that words that hold other positions too can be read, changed and written.  Lanes 4 i .. 4 i + 3 take a group of 32 numbers; the
+// values' codes meet by positions in LDS (`code`: kBlock rows of HD + 4 bytes).
+template <int G>
+__device__ void append_block(const Args &a, int b, int kvh, int pair, int start, int n, int block, uint8_t *code)
+{
+    constexpr int HD = 32 * G, kStride = HD + 4, kWords = (128 * G + kThreads - 1) / kThreads;
+    const int tid = threadIdx.x;
     const int first = block * kBlock - start;   // token of the block's first position
-    if (n == 0 || first >= n) return;
+    const int from = max(0, -first), past = min(kBlock, n - first);
     uint8_t *base = a.cache + ((size_t)pair * a.blocks + block) * (size_t)(1280 * G);
     uint32_t *k_codes = (uint32_t *)base;
     uint32_t *k_scales = (uint32_t *)(base + 512 * G);
     uint32_t *v_codes = (uint32_t *)(base + 640 * G);
     _Float16 *v_scales = (_Float16 *)(base + 1152 * G);
+    const bool whole = past - from == kBlock;
+    uint32_t before[kWords];   // (asked for ahead)
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) before[i] = !whole && tid + i * kThreads < 128 * G ? v_codes[tid + i * kThreads] : 0;
 
-    for (int u = tid; u < kBlock * G * 4; u += kThreads) {
-        const int quad = u % 4, t = u / 4 % G, p = u / (4 * G);
-        const int token = first + p, d = 32 * t + 8 * quad;
-        const bool live = token >= 0 && token < n;
-        const int row = live ? token : 0;
-        const _Float16 *kh = a.k + b * a.k_stride[0] + row * a.k_stride[1] + (size_t)kvh * HD;
-        const _Float16 *vh = a.v + b * a.v_stride[0] + row * a.v_stride[1] + (size_t)kvh * HD;
-        const size_t angle = (size_t)(start + row) * HD;
-        const Held hk = quantise(rotated(kh, a.cos_t + angle, a.sin_t + angle, d, HD));
-        const Held hv = quantise(*(const f16x8 *)(vh + d));
-        if (!live) continue;
+    for (int u = tid; u < (past - from) * G * 4; u += kThreads) {
+        const int quad = u % 4, t = u / 4 % G, p = from + u / (4 * G), token = first + p, d = 32 * t + 8 * quad;
+        const _Float16 *kh = a.k + b * a.k_stride[0] + token * a.k_stride[1] + (size_t)kvh * HD;
+        const _Float16 *vh = a.v + b * a.v_stride[0] + token * a.v_stride[1] + (size_t)kvh * HD;
+        const size_t angle = (size_t)(start + token) * HD;
+        const f16x8 v = *(const f16x8 *)(vh + d);
+        const Held hk = quantise(rotated(kh, a.cos_t + angle, a.sin_t + angle, d, HD)), hv = quantise(v);
         k_codes[(p * 4 + quad) * G + t] = word_of(hk.codes);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) code[p][d + i] = (uint8_t)((hv.codes >> (4 * i)) & 15u);
+        for (int i = 0; i < 8; ++i) code[p * kStride + d + i] = (uint8_t)((hv.codes >> (4 * i)) & 15u);
         if (quad == 0) {
             const f16x2 pair_of = {hk.scale, hk.low};
             k_scales[p * G + t] = __builtin_bit_cast(uint32_t, pair_of);
@@ -185,23 +185,40 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const Args a)
             v_scales[(2 * t) * kBlock + slot] = hv.scale;
             v_scales[(2 * t + 1) * kBlock + slot] = hv.low;
         }
-        const size_t at = ((size_t)b * a.tokens + token) * held_row + (size_t)kvh * HD + d;
+        const size_t at = (((size_t)b * a.tokens + token) * a.kv_heads + kvh) * HD + d;
         if (a.k_held) *(f16x8 *)(a.k_held + at) = hk.value;
         if (a.v_held) *(f16x8 *)(a.v_held + at) = hv.value;
     }
     __syncthreads();
-    for (int u = tid; u < 128 * G; u += kThreads) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        const int u = tid + i * kThreads;
+        if (u >= 128 * G) break;
         const int t = u % (2 * G), column = u / (2 * G) % 16, quad = u / (32 * G);
         uint32_t fresh = 0, mask = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int p = 4 * quad + e % 4 + 16 * (e / 4), shift = 4 * (e / 2) + 16 * (e & 1);
-            if (first + p < 0 || first + p >= n) continue;
-            fresh |= (uint32_t)code[p][16 * t + column] << shift;
+            if (p < from || p >= past) continue;
+            fresh |= (uint32_t)code[p * kStride + 16 * t + column] << shift;
             mask |= 15u << shift;
         }
-        if (mask) v_codes[u] = mask == ~0u ? fresh : (v_codes[u] & ~mask) | fresh;
+        if (mask) v_codes[u] = (before[i] & ~mask) | fresh;
     }
+}
+
+// The new tokens of prompts: one workgroup per block of the cache that they fall into.
+template <int G>
+__global__ void __launch_bounds__(kThreads) append_kernel(const Args a)
+{
+    __shared__ uint8_t code[kBlock * (32 * G + 4)];
+    const int pair = blockIdx.x % a.pairs, part = blockIdx.x / a.pairs;
+    const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
+    int start;
+    const int n = live_tokens(a, b, start);
+    clear_held<32 * G>(a, b, kvh, n, min(part * kBlock, a.tokens), min((part + 1) * kBlock, a.tokens));
+    const int block = start / kBlock + part;
+    if (n > 0 && block * kBlock < start + n) append_block<G>(a, b, kvh, pair, start, n, block, code);
 }
 
 // Two held values from bits 4 I .. of either half of a word (I = 0, 1): the code, put into the low bits of the significand of 1024 (64), is
@@ -333,11 +350,12 @@ __device__ __forceinline__ f16x8 vector_of(const uint32_t (&w)[4]) { return __bu
 // Bound by the stream of the cache: a wave holds a block at a time, the next one's keys are asked for when its scores are formed, its
 // values once they are folded in.
 template <int G, int RT>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const Args a)
+__global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attention_kernel(const Args a)
 {
     constexpr int HD = 32 * G, ROWS = 16 * RT;
     constexpr int kTilesAtOnce = RT == 1 ? 8 : 4;   // of 16 dimensions, joined at a time
     constexpr int kPadded = 16 * kTilesAtOnce + 4;
+    static_assert(sizeof(float) * kWaves * ROWS * kPadded >= kBlock * (HD + 4), "room for an appended block");
     __shared__ float joined[kWaves][ROWS][kPadded];
     __shared__ float2 wave_stats[kWaves][ROWS];
 
@@ -354,7 +372,16 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Args a)
     const int blocks = (limit_high + kBlock) / kBlock;
     const int per = blocks_per_split(a, blocks, kWaves);
     const int begin = split * per, end = min(begin + per, blocks);
+    if (a.fused && split == 0) clear_held<HD>(a, b, kvh, n, 0, a.tokens);
     if (a.splits > 1 && begin >= end) return;                                  // (nobody reads its part)
+
+    // Fused: the one tile of a pair's rows; the workgroup whose blocks new tokens fall into appends them before anything is read.
+    if (a.fused && n > 0 && start / kBlock < end) {
+        for (int fresh = max(start / kBlock, begin); fresh < end; ++fresh) {
+            append_block<G>(a, b, kvh, pair, start, n, fresh, (uint8_t *)joined);
+            __syncthreads();
+        }
+    }
 
     f16x8 q[RT][G];
     int limit[RT];
@@ -661,23 +688,29 @@ int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int 
     if (heads < kv_heads || heads > 4096 || heads % kv_heads != 0) return LUTGEMM_EINVAL;
     const long rows = (long)tokens * (heads / kv_heads), pairs = (long)batch * kv_heads;
     const int blocks = (max_positions + kBlock - 1) / kBlock;
-    p->fused = 0;
+    // (one tile of rows per pair: its workgroups append themselves, a launch and 8 us less for single tokens)
+    p->fused = rows <= 32;
     p->rows_per_wave = rows > 16 ? 32 : 16;
     p->rows_apart = rows >= 4 * 32;
-    const int waves = p->rows_apart && rows < 8 * 32 ? 4 : p->rows_apart ? 8 : kWaves;
+    // (eight waves share the forming of a block, where that leaves a workgroup for every CU)
+    const int waves = p->rows_apart && pairs * ((rows + 8 * 32 - 1) / (8 * 32)) >= 256 ? 8 : 4;
     p->threads = 64 * waves;
     s->units = (int)((rows + p->rows_per_wave - 1) / p->rows_per_wave);
     s->tiles = p->rows_apart ? (s->units + waves - 1) / waves : s->units;
     const long alone = pairs * s->tiles;
+    // Positions are shared by workgroups where the CUs hold more of them at once than there are tiles, and a wave would have more than ten
+    // blocks to itself: the joining launch takes 4 to 5 us, a block about half of one (8 sequences of 32 heads at position 1023: one 16.3 us, two
+    // 20 us; one of 8 at 8191: one 33 us, 32 12.4 us; 24 of 8, up to 4096: one 27.7 us, four 18.9 us).
     long splits = 1;
-    if (alone * waves < 4096) splits = (4096 + alone * waves - 1) / (alone * waves);
-    const long most = blocks / 32;   // each split has some blocks to itself
+    const long room = (p->rows_apart ? 512 : 768) * 4 / (alone * waves);
+    if (blocks > (p->rows_apart ? 32 : 10 * waves)) splits = room;
+    const long most = blocks / (p->rows_apart ? 16 : 2 * waves);   // each has some blocks to itself
     if (splits > most) splits = most;
     if (splits > kMostSplits) splits = kMostSplits;
     if (splits < 1) splits = 1;
     p->splits = (int)splits;
     p->row_tiles = s->tiles;
-    p->launches = splits > 1 ? 3 : 2;
+    p->launches = 1 + !p->fused + (splits > 1);
     if (alone * splits > 0x7fffffffl || pairs * ((tokens + kBlock - 1) / kBlock + 1) > 0x7fffffffl) return LUTGEMM_EINVAL;
     p->workgroups = (int)(alone * splits);
     const size_t part_rows = (size_t)splits * pairs * s->units * p->rows_per_wave;
@@ -759,16 +792,20 @@ int lutgemm_q4_attention_f16(const lutgemm_q4_attention *c, void *workspace, siz
     a.units = sizes.units;
     a.tiles = sizes.tiles;
     a.splits = plan.splits;
+    a.fused = plan.fused;
     a.partial = (float *)workspace;
     a.stats = (float2 *)((float *)workspace + sizes.partial_floats);
     const hipStream_t hs = (hipStream_t)stream;
 
     auto run = [&](auto g_c) -> int {
         constexpr int G = decltype(g_c)::value;
-        const long parts = (a.tokens + kBlock - 1) / kBlock + 1;
-        hipLaunchKernelGGL(append_kernel<G>, dim3((unsigned)(parts * a.pairs)), dim3(kThreads), 0, hs, a);
-        int status = launch_status();
-        if (status != LUTGEMM_OK) return status;
+        int status = LUTGEMM_OK;
+        if (!plan.fused) {
+            const long parts = (a.tokens + kBlock - 1) / kBlock + 1;
+            hipLaunchKernelGGL(append_kernel<G>, dim3((unsigned)(parts * a.pairs)), dim3(kThreads), 0, hs, a);
+            status = launch_status();
+            if (status != LUTGEMM_OK) return status;
+        }
         const dim3 grid((unsigned)plan.workgroups), threads((unsigned)plan.threads);
         if (plan.rows_apart && plan.threads == 512) hipLaunchKernelGGL((prompt_kernel<G, 8>), grid, threads, 0, hs, a);
         else if (plan.rows_apart) hipLaunchKernelGGL((prompt_kernel<G, 4>), grid, threads, 0, hs, a);
