@@ -279,18 +279,17 @@ struct RowState {
 #pragma unroll
         for (int t = 0; t < 2 * G; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // The weights of a block's scores (half h of the block: positions j0 + 16 h + 4 quad + i); `edge`: some may lie behind `limit`.
-    __device__ __forceinline__ f16x8 weights(const f32x4 (&score)[2], float factor, bool edge, int j0, int limit)
+    // The reference raised for a block's scores where they call for it (half h of the block: positions j0 + 16 h + 4 quad + i); `edge`:
+    // some may lie behind `limit`, and become -inf.
+    __device__ __forceinline__ void raise(f32x4 (&score)[2], float factor, bool edge, int j0, int limit)
     {
         const int quad = (threadIdx.x & 63) >> 4;
-        float s[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = score[e / 4][e % 4];
         if (edge) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = j0 + 16 * (e / 4) + 4 * quad + e % 4 <= limit ? s[e] : -INFINITY;
+            for (int e = 0; e < 8; ++e) score[e / 4][e % 4] = j0 + 16 * (e / 4) + 4 * quad + e % 4 <= limit ? score[e / 4][e % 4] : -INFINITY;
         }
-        float most = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        const f32x4 s = score[0], u = score[1];
+        float most = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])));
         if (__any((most - reference) * factor > kSlack)) {
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
@@ -300,11 +299,14 @@ struct RowState {
 #pragma unroll
             for (int t = 0; t < 2 * G; ++t) acc[t] *= keep;
         }
+    }
+    __device__ __forceinline__ f16x8 weights(const f32x4 (&score)[2], float factor)
+    {
         const float off = -reference * factor;
         f16x8 w;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[e], factor, off));
+            const float p = __builtin_amdgcn_exp2f(fmaf(score[e / 4][e % 4], factor, off));
             sum += p;
             w[e] = (_Float16)p;
         }
@@ -434,7 +436,10 @@ __global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attenti
         const bool edge = j0 + kBlock - 1 > limit_low;
         f16x8 weight[RT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) weight[rt] = state[rt].weights(score[rt], factor, edge, j0, limit[rt]);
+        for (int rt = 0; rt < RT; ++rt) {
+            state[rt].raise(score[rt], factor, edge, j0, limit[rt]);
+            weight[rt] = state[rt].weights(score[rt], factor);
+        }
         if (j0 + kBlock - 1 > limit_high) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -496,14 +501,19 @@ __global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attenti
     }
 }
 
-// Many query rows (prompts): the waves of a workgroup take 32 rows each, side by side, and all of its blocks together.  A block's keys and
+// Many query rows (prompts): the waves of a workgroup take 16 RT rows each, side by side, and all of its blocks together.  A block's keys and
 // values are formed once for all waves, by pieces, and handed over through LDS as the matrix instructions' operands: a wave that forms them for
 // itself does nothing else for most of its time (two prompts of 2048 tokens, 32 heads on 8: 197 us, vector unit 62 % busy, matrix unit 15 %).
-// Two buffers, one barrier a block: while a block is multiplied, the next one is formed and the one behind it asked for.
+// Two buffers each, one barrier a block.  In the time of a block its weights are formed while the next block's scores are multiplied, from keys
+// that stand ready, and its values multiplied while the pieces of later blocks are formed; operands are read from LDS all at once, ahead of
+// their use (read one at a time, each wave waited for each: 107 us for those prompts).
+template <int G>
+constexpr int kPromptTiles = G > 4 ? 1 : 2;   // tiles of 16 rows a wave takes, as registers allow
+
 template <int G, int W>
-__global__ void __launch_bounds__(64 * W) prompt_kernel(const Args a)
+__global__ void __launch_bounds__(64 * W, 2) prompt_kernel(const Args a)
 {
-    constexpr int HD = 32 * G, RT = 2, ROWS = 16 * RT;
+    constexpr int HD = 32 * G, RT = kPromptTiles<G>, ROWS = 16 * RT;
     constexpr int kPieces = (2 * G + W - 1) / W;   // of 2 G operands of keys and as many of values, a wave's
     __shared__ f16x8 keys[2][2 * G][64], values[2][2 * G][64];
 
@@ -526,27 +536,41 @@ __global__ void __launch_bounds__(64 * W) prompt_kernel(const Args a)
 
     const uint8_t *cache = a.cache + (size_t)pair * a.blocks * (size_t)(1280 * G);
     uint32_t k_code[kPieces], k_scale[kPieces], v_code[kPieces], v_scale[kPieces][2][4];
-    auto fetch = [&](int block) {
+    auto mine = [&](int i) { return 2 * G % W == 0 || wave + i * W < 2 * G; };
+    auto fetch_keys = [&](int block) {
         const uint8_t *base = cache + (size_t)block * (1280 * G);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int f = wave + i * W, position = 16 * (f / G) + column;
-            if (2 * G % W != 0 && f >= 2 * G) continue;
+            if (!mine(i)) continue;
             k_code[i] = *(const uint32_t *)(base + ((position * 4 + quad) * G + f % G) * 4);
             k_scale[i] = *(const uint32_t *)(base + 512 * G + (position * G + f % G) * 4);
+        }
+    };
+    auto fetch_values = [&](int block) {
+        const uint8_t *base = cache + (size_t)block * (1280 * G);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int f = wave + i * W;
+            if (!mine(i)) continue;
             v_code[i] = *(const uint32_t *)(base + 640 * G + ((quad * 16 + column) * 2 * G + f) * 4);
             load_words(v_scale[i][0], base + 1152 * G + (f & ~1) * 64 + quad * 16);
             load_words(v_scale[i][1], base + 1152 * G + (f | 1) * 64 + quad * 16);
         }
     };
-    auto form = [&](int block, int buffer) {
+    auto form_keys = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            if (!mine(i)) continue;
+            const f16x2 sm = __builtin_bit_cast(f16x2, k_scale[i]);
+            keys[buffer][wave + i * W][lane] = __builtin_elementwise_fma(codes_of(k_code[i]), (f16x8)(sm.x), (f16x8)(sm.y));
+        }
+    };
+    auto form_values = [&](int block, int buffer) {
         const bool beyond = (block + 1) * kBlock - 1 > tile_high;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int f = wave + i * W;
-            if (2 * G % W != 0 && f >= 2 * G) continue;
-            const f16x2 sm = __builtin_bit_cast(f16x2, k_scale[i]);
-            keys[buffer][f][lane] = __builtin_elementwise_fma(codes_of(k_code[i]), (f16x8)(sm.x), (f16x8)(sm.y));
+            if (!mine(i)) continue;
             if (beyond) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -555,10 +579,15 @@ __global__ void __launch_bounds__(64 * W) prompt_kernel(const Args a)
                     v_scale[i][1][j] &= mask;
                 }
             }
-            values[buffer][f][lane] = __builtin_elementwise_fma(codes_of(v_code[i]), vector_of(v_scale[i][0]), vector_of(v_scale[i][1]));
+            values[buffer][wave + i * W][lane] = __builtin_elementwise_fma(codes_of(v_code[i]), vector_of(v_scale[i][0]), vector_of(v_scale[i][1]));
         }
     };
-    if (begin < end) fetch(begin);
+    // (blocks behind the last are asked for and formed like it, and not used: no branch in the loop)
+    auto inside = [&](int block) { return min(block, end - 1); };
+    if (begin < end) {
+        fetch_keys(begin);
+        fetch_values(begin);
+    }
     f16x8 q[RT][G];
     int limit[RT];
     load_queries<G, RT>(a, b, kvh, start, row0, live_rows, q, limit);
@@ -566,41 +595,72 @@ __global__ void __launch_bounds__(64 * W) prompt_kernel(const Args a)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) state[rt].clear();
     const float factor = 1.4426950408889634f / sqrtf((float)HD);
-    if (begin < end) {
-        form(begin, 0);
-        if (begin + 1 < end) fetch(begin + 1);
-    }
-    for (int block = begin; block < end; ++block) {
-        const int buffer = (block - begin) & 1;
-        __syncthreads();   // this block is formed, and the other buffer read
-        if (block + 1 < end) {
-            form(block + 1, buffer ^ 1);
-            if (block + 2 < end) fetch(block + 2);
-        }
-        if (block >= own_end) continue;
-        f32x4 score[RT][2];
+    f32x4 score[RT][2];
+    f16x8 operand[2 * G];
+    auto multiply_keys = [&](f32x4 (&to)[RT][2]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) score[rt][h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int rt = 0; rt < RT; ++rt) to[rt][h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int t = 0; t < G; ++t) {
-                const f16x8 key = keys[buffer][h * G + t][lane];
+            for (int t = 0; t < G; ++t)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) score[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[rt][t], score[rt][h], 0, 0, 0);
+                for (int rt = 0; rt < RT; ++rt) to[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand[h * G + t], q[rt][t], to[rt][h], 0, 0, 0);
+        }
+    };
+    if (begin < end) {
+        form_keys(0);
+        form_values(begin, 0);
+        fetch_keys(inside(begin + 1));
+        fetch_values(inside(begin + 1));
+        __syncthreads();
+#pragma unroll
+        for (int f = 0; f < 2 * G; ++f) operand[f] = keys[0][f][lane];
+        multiply_keys(score);
+        form_keys(1);
+        fetch_keys(inside(begin + 2));
+    }
+    for (int block = begin; block < end; ++block) {
+        const int buffer = (block - begin) & 1;
+        // Here: this block's scores in registers, its values formed, the next one's keys formed; its values' codes and the keys' of the one
+        // after it in registers.
+        __syncthreads();
+        if (block < own_end) {
+#pragma unroll
+            for (int f = 0; f < 2 * G; ++f) operand[f] = keys[buffer ^ 1][f][lane];
+            __builtin_amdgcn_sched_barrier(0);
+            const int j0 = block * kBlock;
+            const bool edge = j0 + kBlock - 1 > limit_low;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) state[rt].raise(score[rt], factor, edge, j0, limit[rt]);
+            f32x4 next[RT][2];
+            f16x8 weight[RT];
+            multiply_keys(next);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) weight[rt] = state[rt].weights(score[rt], factor);
+#pragma unroll
+            for (int i = 0; i < 2 * G * RT; ++i) {   // a matrix instruction, then vector ones in its time
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x402, 3, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < 2 * G; ++f) operand[f] = values[buffer][f][lane];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < 2 * G; ++t)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) state[rt].acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand[t], weight[rt], state[rt].acc[t], 0, 0, 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                score[rt][0] = next[rt][0];
+                score[rt][1] = next[rt][1];
             }
         }
-        const int j0 = block * kBlock;
-        const bool edge = j0 + kBlock - 1 > limit_low;
-        f16x8 weight[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) weight[rt] = state[rt].weights(score[rt], factor, edge, j0, limit[rt]);
-#pragma unroll
-        for (int t = 0; t < 2 * G; ++t) {
-            const f16x8 value = values[buffer][t][lane];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) state[rt].acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weight[rt], state[rt].acc[t], 0, 0, 0);
-        }
+        form_keys(buffer);
+        form_values(inside(block + 1), buffer ^ 1);
+        fetch_keys(inside(block + 3));
+        fetch_values(inside(block + 2));
     }
     if (unit >= a.units) return;
 #pragma unroll
@@ -690,10 +750,12 @@ int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int 
     const int blocks = (max_positions + kBlock - 1) / kBlock;
     // (one tile of rows per pair: its workgroups append themselves, a launch and 8 us less for single tokens)
     p->fused = rows <= 32;
-    p->rows_per_wave = rows > 16 ? 32 : 16;
     p->rows_apart = rows >= 4 * 32;
-    // (eight waves share the forming of a block, where that leaves a workgroup for every CU)
-    const int waves = p->rows_apart && pairs * ((rows + 8 * 32 - 1) / (8 * 32)) >= 256 ? 8 : 4;
+    p->rows_per_wave = rows > 16 && !(p->rows_apart && head_dim > 128) ? 32 : 16;
+    // (eight waves share the forming of a block, where that leaves a workgroup for every CU: a prompt of 512 on 32 kv heads by fours 37.8 us, by
+    // eights 44; a chunk of 256 of 32 heads on 8 kv heads onto 30000 positions, whose positions are shared, 210 and 187)
+    const long eights = pairs * ((rows + 8 * p->rows_per_wave - 1) / (8 * p->rows_per_wave)) * (blocks > 32 ? blocks / 16 : 1);
+    const int waves = p->rows_apart && eights >= 256 ? 8 : 4;
     p->threads = 64 * waves;
     s->units = (int)((rows + p->rows_per_wave - 1) / p->rows_per_wave);
     s->tiles = p->rows_apart ? (s->units + waves - 1) / waves : s->units;
