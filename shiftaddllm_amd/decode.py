@@ -20,6 +20,10 @@ default) runs this library's fused kernels -- RMSNorm, rotary + KV append +
 attention, SiLU*up -- and lets o_proj / down_proj accumulate straight into the
 residual stream, eight launches per block (five with grouped launches); glue="torch" spells the same step in
 framework operations and is what the parity test's dense model is built from.
+
+Beyond the reference's protocol the decoder can hold its cache in 4 bits (kv_bits=4: every sequence then stands at a
+position of its own, and prompts are taken at once by prefill()), run low-rank adapters of many requests beside its
+linears (adapters=(count, rank)) and draw its tokens (sampling=SamplingOptions(...)).
 """
 from __future__ import annotations
 
@@ -34,7 +38,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import native
+from .kv_cache import Q4Cache
+from .lut_gemm.adapters import AdapterBank
 from .lut_gemm.quant import LutLinear
+from .sampling import SamplingOptions
 
 
 @dataclass
@@ -87,6 +94,9 @@ class Block(nn.Module):
         self.input_norm = nn.Parameter(torch.ones(h, dtype=torch.float16, device=device))
         self.post_norm = nn.Parameter(torch.ones(h, dtype=torch.float16, device=device))
 
+    def linears(self):
+        return self.q_proj, self.k_proj, self.v_proj, self.o_proj, self.gate_proj, self.up_proj, self.down_proj
+
 
 def rms_norm(x, w, eps):
     xf = x.float()
@@ -94,14 +104,29 @@ def rms_norm(x, w, eps):
 
 
 class LutDecoder(nn.Module):
-    """Single-token-per-step decoder with a static KV cache of cfg.max_positions."""
+    """Single-token-per-step decoder with a static KV cache of cfg.max_positions.
+
+    kv_bits=4 (glue="hip" only): the cache is held in 4 bits (self.q4, a Q4Cache per block), and forward_token takes a
+    position for every sequence; a negative one leaves that sequence idle.
+    adapters=(count, rank): every linear gets an AdapterBank of zeros (`lin.adapters`, to be filled); self.adapter_ids, int32
+    [batch], names each sequence's adapter, -1 for none.
+    sampling: a step ends by drawing a token per sequence from its logits with self.uniform, float32 [batch], into
+    self.next_ids and self.next_logprob.  self.sample_temperature, _top_k, _top_p and _min_p hold the options per sequence."""
 
     def __init__(self, cfg: DecoderConfig, quant_config: dict | None = None, batch: int = 1, seed: int = 0,
                  device="cuda:0", default_bits: int = 3, fuse_launches: bool = True,
-                 module_prefix: str = "model.layers", glue: str = "hip", chain: bool = False):
+                 module_prefix: str = "model.layers", glue: str = "hip", chain: bool = False, kv_bits: int = 16,
+                 adapters: tuple[int, int] | None = None, sampling: SamplingOptions | None = None):
         super().__init__()
         if glue not in ("hip", "torch"):
             raise ValueError(f"glue must be 'hip' or 'torch', got {glue!r}")
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, got {kv_bits}")
+        if kv_bits == 4 and glue != "hip":
+            raise ValueError("a cache of 4 bits needs glue='hip'")
+        if chain and (kv_bits == 4 or adapters is not None):
+            raise ValueError("chained launches run with the fp16 cache and without adapters")
+        self.kv_bits, self.sampling, self.has_adapters = kv_bits, sampling, adapters is not None
         self.cfg, self.batch, self.fuse, self.glue = cfg, batch, fuse_launches, glue
         # o_proj, gate/up, down_proj and the next block's q,k,v as ONE chained launch per block (tagged
         # rows hand the activations over inside the launch): two launches per block with the attention
@@ -124,6 +149,9 @@ class LutDecoder(nn.Module):
             bits = {n: (quant_config or {}).get(f"{module_prefix}.{i}.{n}", {}).get("bits", default_bits)
                     for n in names}
             self.blocks.append(Block(cfg, bits, gen, dev))
+            if adapters is not None:
+                for l in self.blocks[-1].linears():
+                    l.adapters = AdapterBank(l.K, l.N, adapters[1], adapters[0]).to(dev)
         scale = 0.02
         self.embed = nn.Parameter((torch.randn((cfg.vocab_size, cfg.hidden), generator=gen, device=dev) * scale).half())
         self.lm_head = nn.Parameter((torch.randn((cfg.vocab_size, cfg.hidden), generator=gen, device=dev) * scale).half())
@@ -134,8 +162,22 @@ class LutDecoder(nn.Module):
         self.register_buffer("cos", torch.cat([ang.cos(), ang.cos()], dim=-1).half(), persistent=False)
         self.register_buffer("sin", torch.cat([ang.sin(), ang.sin()], dim=-1).half(), persistent=False)
         shape = (cfg.layers, batch, cfg.kv_heads, cfg.max_positions, hd)
-        self.register_buffer("k_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
-        self.register_buffer("v_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
+        if kv_bits == 16:
+            self.register_buffer("k_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
+            self.register_buffer("v_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
+        else:
+            self.q4 = [Q4Cache(batch, cfg.kv_heads, cfg.max_positions, hd, dev) for _ in range(cfg.layers)]
+            self.register_buffer("starts", torch.zeros((batch,), dtype=torch.long, device=dev), persistent=False)
+        if adapters is not None:
+            self.register_buffer("adapter_ids", torch.full((batch,), -1, dtype=torch.int32, device=dev), persistent=False)
+        if sampling is not None:
+            full = lambda v, t: torch.full((batch,), v, dtype=t, device=dev)
+            for name, t in (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32), ("min_p", torch.float32)):
+                self.register_buffer("sample_" + name, full(getattr(sampling, name), t), persistent=False)
+            self.register_buffer("uniform", full(0.0, torch.float32), persistent=False)
+            self.register_buffer("next_ids", full(0, torch.long), persistent=False)
+            self.register_buffer("next_logprob", full(0.0, torch.float32), persistent=False)
+        self._workspaces = []                                  # of adapters and sampling, see _workspace
         self.register_buffer("positions", torch.arange(cfg.max_positions, device=dev), persistent=False)
         # static step inputs/outputs (graph replay reads and writes these)
         self.register_buffer("ids", torch.zeros((batch,), dtype=torch.long, device=dev), persistent=False)
@@ -160,7 +202,7 @@ class LutDecoder(nn.Module):
             self.register_buffer("up_tagged", torch.zeros((batch, I), **i32), persistent=False)
             self.register_buffer("chain_words", torch.zeros((2,), **i32), persistent=False)   # epoch, status
         # what a step reads besides the KV cache: the attention kernel reads past the caches where it is much
-        self.step_bytes = sum(t.nbytes for t in self.blocks.buffers()) + self.lm_head.nbytes
+        self.step_bytes = sum(t.nbytes for n, t in self.blocks.named_buffers() if ".adapters." not in n) + self.lm_head.nbytes
         self._graph = None
         self._stream = None
 
@@ -187,6 +229,8 @@ class LutDecoder(nn.Module):
         return outs
 
     def _linears(self, lins, x):
+        if self.has_adapters:
+            return [l(x, self.adapter_ids) for l in lins]
         if self.fuse and len(lins) > 1:
             return self._fused(lins, x)
         return [l(x) for l in lins]
@@ -199,10 +243,145 @@ class LutDecoder(nn.Module):
     # ---- one token ---------------------------------------------------------------------------
     @torch.no_grad()
     def step(self):
-        """Consumes self.ids [B] at position self.pos [1]; writes self.logits [B, V]."""
-        if self.glue == "hip":
-            return self._step_hip()
-        return self._step_torch()
+        """Consumes self.ids [B] at position self.pos [1] (self.starts [B] with a cache of 4 bits); writes self.logits [B, V]
+        and, with sampling, self.next_ids and self.next_logprob [B]."""
+        if self.glue == "torch":
+            self._step_torch()
+        elif self.has_adapters:
+            self._step_adapted()
+        else:
+            self._step_hip()
+        if self.sampling is not None:
+            self._draw()
+
+    def _workspace(self, size):
+        """Device memory for one call at a time of this decoder's stream.  (What was outgrown is kept: a captured step names it.)"""
+        if not self._workspaces or self._workspaces[-1].numel() < size:
+            self._workspaces.append(torch.empty(size, dtype=torch.uint8, device=self.logits.device))
+        return self._workspaces[-1].data_ptr()
+
+    def _draw(self):
+        lib = native.cabi()
+        B, V = self.logits.shape
+        size = lib.lutgemm_sampling_workspace(B, V)
+        call = native.Sampling(self.logits.data_ptr(), V, 0, B, V, self.sample_temperature.data_ptr(), self.sample_top_k.data_ptr(),
+                               self.sample_top_p.data_ptr(), self.sample_min_p.data_ptr(), self.uniform.data_ptr(),
+                               self.next_ids.data_ptr(), self.next_logprob.data_ptr())
+        rc = lib.lutgemm_sample_tokens(ctypes.byref(call), self._workspace(size), size, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        if rc:
+            raise RuntimeError(lib.lutgemm_strerror(rc).decode())
+
+    def _adapt(self, lins, x, outs, sp):
+        """outs[i] += the adapters of lins[i] on x, row by row; the linears share two launches."""
+        lib, M = native.cabi(), x.shape[0]
+        arr = (native.Adapters * len(lins))()
+        for i, (l, o) in enumerate(zip(lins, outs)):
+            a = l.adapters
+            arr[i] = native.Adapters(x.data_ptr(), o.data_ptr(), o.data_ptr(), self.adapter_ids.data_ptr(), a.down.data_ptr(), a.up.data_ptr(),
+                                     a.scale.data_ptr(), l.K, l.N, l.N, M, l.N, l.K, a.rank, a.count)
+        size = lib.lutgemm_adapters_workspace(len(lins), arr)
+        rc = lib.lutgemm_adapters_f16(len(lins), arr, self._workspace(size), size, sp)
+        if rc:
+            raise RuntimeError(lib.lutgemm_strerror(rc).decode())
+
+    def _attention(self, li, q, k, v, sp):
+        """self.att = attention of the new tokens' queries in block li, their keys and values appended."""
+        cfg, B = self.cfg, self.batch
+        if self.kv_bits == 4:
+            self.q4[li].attend(q.view(B, -1), k.view(B, -1), v.view(B, -1), self.cos, self.sin, self.starts, out=self.att)
+            return
+        lib = native.cabi()
+        rc = lib.lutgemm_decode_attention_step_f16(q.data_ptr(), k.data_ptr(), v.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(),
+                                                   self.k_cache[li].data_ptr(), self.v_cache[li].data_ptr(), self.pos.data_ptr(),
+                                                   self.att.data_ptr(), B, cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.max_positions,
+                                                   self.step_bytes, sp)
+        if rc:
+            raise RuntimeError(lib.lutgemm_strerror(rc).decode())
+
+    def _step_adapted(self):
+        """glue="hip" with adapters: they read the linears' inputs, so the norms and SiLU*up around them are launches of their own."""
+        cfg, B = self.cfg, self.batch
+        hd, H, KV, I = cfg.head_dim, cfg.heads, cfg.kv_heads, cfg.intermediate
+        lib = native.cabi()
+        sp = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+        def check(rc):
+            if rc:
+                raise RuntimeError(lib.lutgemm_strerror(rc).decode())
+
+        def linears(lins, x, outs, overwrite=True):
+            if self.fuse:
+                self._fused_gemv(lins, x, outs, sp, overwrite=overwrite)
+            else:
+                for l, o in zip(lins, outs):
+                    self._fused_gemv([l], x, [o], sp, overwrite=overwrite)
+            self._adapt(lins, x, outs, sp)
+
+        nq, nkv = B * H * hd, B * KV * hd
+        q, k, v = self.qkv[:nq], self.qkv[nq:nq + nkv], self.qkv[nq + nkv:]
+        g, u = self.gate_up[:B * I].view(B, I), self.gate_up[B * I:].view(B, I)
+        x, h = self.x_res, self.h_norm
+        rmsnorm = lambda w: check(lib.lutgemm_decode_rmsnorm_f16(x.data_ptr(), w.data_ptr(), h.data_ptr(), B, cfg.hidden, cfg.rms_eps, None, 0, sp))
+        torch.index_select(self.embed, 0, self.ids, out=x)
+        for li, blk in enumerate(self.blocks):
+            rmsnorm(blk.input_norm)
+            linears([blk.q_proj, blk.k_proj, blk.v_proj], h, [q, k, v])
+            self._attention(li, q, k, v, sp)
+            linears([blk.o_proj], self.att, [x], overwrite=False)
+            rmsnorm(blk.post_norm)
+            linears([blk.gate_proj, blk.up_proj], h, [g, u])
+            check(lib.lutgemm_decode_silu_mul_f16(g.data_ptr(), u.data_ptr(), self.act.data_ptr(), B * I, sp))
+            linears([blk.down_proj], self.act, [x], overwrite=False)
+        rmsnorm(self.final_norm)
+        torch.matmul(h, self.lm_head.t(), out=self.logits)
+
+    @torch.no_grad()
+    def prefill(self, input_ids: torch.Tensor, lengths=None, starts=None):
+        """Takes prompts at once (cache of 4 bits): input_ids [batch, T], of which lengths[b] tokens are there (None: all), the first at
+        position starts[b] (None: 0).  Leaves the logits behind each sequence's last token in self.logits and returns them; a
+        sequence without tokens keeps the logits that were there."""
+        if self.kv_bits != 4:
+            raise ValueError("prefill needs a cache of 4 bits (kv_bits=4); the fp16 cache takes one token at a time")
+        cfg, dev = self.cfg, self.logits.device
+        B, T = input_ids.shape
+        lengths = [T] * B if lengths is None else [int(n) for n in lengths]
+        starts = [0] * B if starts is None else [int(p) for p in starts]
+        if B != self.batch or T < 1 or len(lengths) != B or len(starts) != B:
+            raise ValueError(f"input_ids must be [{self.batch}, T] with a length and a start for each sequence")
+        for n, p in zip(lengths, starts):
+            if not 0 <= n <= T or (n > 0 and not 0 <= p <= cfg.max_positions - n):
+                raise ValueError(f"{n} tokens at position {p} outside the KV cache of {cfg.max_positions} positions")
+        start = torch.tensor(starts, device=dev)
+        count = torch.tensor(lengths, dtype=torch.int32, device=dev)
+        ids = self.adapter_ids.repeat_interleave(T) if self.has_adapters else None
+        lib = native.cabi()
+        sp = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+        def check(rc):
+            if rc:
+                raise RuntimeError(lib.lutgemm_strerror(rc).decode())
+
+        def norm(x, w):
+            h = torch.empty_like(x)
+            check(lib.lutgemm_decode_rmsnorm_f16(x.data_ptr(), w.data_ptr(), h.data_ptr(), x.shape[0], cfg.hidden, cfg.rms_eps, None, 0, sp))
+            return h
+
+        x = self.embed[input_ids.to(dev).reshape(-1)]
+        for li, blk in enumerate(self.blocks):
+            h = norm(x, blk.input_norm)
+            q, k, v = (l(h, ids).view(B, T, -1) for l in (blk.q_proj, blk.k_proj, blk.v_proj))
+            att = self.q4[li].attend(q, k, v, self.cos, self.sin, start, count)
+            x = x + blk.o_proj(att.view(B * T, -1), ids)
+            h = norm(x, blk.post_norm)
+            g, u = blk.gate_proj(h, ids), blk.up_proj(h, ids)
+            act = torch.empty_like(g)
+            check(lib.lutgemm_decode_silu_mul_f16(g.data_ptr(), u.data_ptr(), act.data_ptr(), g.numel(), sp))
+            x = x + blk.down_proj(act, ids)
+        some = [b for b in range(B) if lengths[b] > 0]
+        if some:
+            rows = torch.tensor([b * T + lengths[b] - 1 for b in some], device=dev)
+            self.logits[torch.tensor(some, device=dev)] = norm(x[rows], self.final_norm) @ self.lm_head.t()
+        return self.logits
 
     def _gemv_into(self, lins, x, outs, sp):
         """outs[i] += lins[i](x); one grouped launch when fusing."""
@@ -336,11 +515,7 @@ class LutDecoder(nn.Module):
             else:
                 rmsnorm(blk.input_norm, self.qkv)
                 self._gemv_into(qkv_lins, h, [q, k, v], sp)
-            check(lib.lutgemm_decode_attention_step_f16(q.data_ptr(), k.data_ptr(), v.data_ptr(), self.cos.data_ptr(),
-                                                        self.sin.data_ptr(), self.k_cache[li].data_ptr(),
-                                                        self.v_cache[li].data_ptr(), self.pos.data_ptr(),
-                                                        self.att.data_ptr(), B, H, KV, hd, cfg.max_positions,
-                                                        self.step_bytes, sp))
+            self._attention(li, q, k, v, sp)
             gate_up, act = [blk.gate_proj, blk.up_proj], None if fold_gate else self.act
             if split:                                                   # x += o_proj(att); h = x * post_norm
                 self._fused_gemv([blk.o_proj], self.att, [x], sp, next_norm=blk.post_norm, next_in=h,
@@ -418,13 +593,24 @@ class LutDecoder(nn.Module):
         self._graph = g
 
     @torch.no_grad()
-    def forward_token(self, ids: torch.Tensor, position: int):
-        # the attention kernel clamps the position into the cache: past its end it would
-        # overwrite the last slot and return plausible but wrong logits
-        if not 0 <= position < self.cfg.max_positions:
-            raise ValueError(f"position {position} outside the KV cache of {self.cfg.max_positions} positions")
+    def forward_token(self, ids: torch.Tensor, position):
+        """One token per sequence at `position`; with a cache of 4 bits also a position for every sequence (a list or a tensor in
+        host memory), negative for one that is idle."""
+        P = self.cfg.max_positions
+        if isinstance(position, int):
+            # the attention kernel clamps the position into the cache: past its end it would
+            # overwrite the last slot and return plausible but wrong logits
+            if not 0 <= position < P:
+                raise ValueError(f"position {position} outside the KV cache of {P} positions")
+            (self.pos if self.kv_bits == 16 else self.starts).fill_(position)
+        else:
+            positions = [int(p) for p in position]
+            if self.kv_bits != 4:
+                raise ValueError("the fp16 cache takes one position for all sequences")
+            if len(positions) != self.batch or any(p >= P for p in positions):
+                raise ValueError(f"{self.batch} positions inside the KV cache of {P} positions are needed, got {positions}")
+            self.starts.copy_(torch.tensor(positions))
         self.ids.copy_(ids)
-        self.pos.fill_(position)
         if self._graph is not None:
             self._graph.replay()
         else:
@@ -432,6 +618,10 @@ class LutDecoder(nn.Module):
         return self.logits
 
     def reset(self):
+        if self.kv_bits == 4:
+            for cache in self.q4:
+                cache.data.zero_()
+            return
         self.k_cache.zero_()
         self.v_cache.zero_()
 
@@ -454,7 +644,8 @@ def benchmark(model: LutDecoder, input_ids: torch.Tensor, generate: int = 128, w
     (batch * 1/median) and the generated ids.  With `check` the cross-entropy of every
     prompt position's logits against the next prompt token is accumulated as well and
     `ppl` = exp(mean loss) is returned, as model/opt.py:382-384,414-423 does (outside
-    the timed region of a token)."""
+    the timed region of a token).  A decoder with sampling draws its tokens instead of taking the most
+    likely ones, in the step itself, with random numbers from its options' seed."""
     B, T = input_ids.shape
     assert B == model.batch and T + generate <= model.cfg.max_positions
     dev = model.ids.device
@@ -466,8 +657,11 @@ def benchmark(model: LutDecoder, input_ids: torch.Tensor, generate: int = 128, w
     times_prompt, times_gen, out_ids = [], [], []
     nxt = None
     tot = torch.zeros((), dtype=torch.float32, device=dev)
+    numbers = torch.Generator(device=dev).manual_seed(model.sampling.seed) if model.sampling is not None else None
     for i in range(T + generate):
         ids = input_ids[:, i] if i < T else nxt
+        if numbers is not None:
+            model.uniform.copy_(torch.rand(B, generator=numbers, device=dev))
         torch.cuda.synchronize()
         tick = time.perf_counter()
         logits = model.forward_token(ids, i)
@@ -475,7 +669,7 @@ def benchmark(model: LutDecoder, input_ids: torch.Tensor, generate: int = 128, w
         (times_prompt if i < T else times_gen).append(time.perf_counter() - tick)
         if check and i < T - 1:
             tot += F.cross_entropy(logits.float(), input_ids[:, i + 1])
-        nxt = logits.argmax(dim=-1)
+        nxt = logits.argmax(dim=-1) if numbers is None else model.next_ids.clone()
         if i >= T - 1:
             out_ids.append(nxt.clone())
     med = statistics.median(times_gen) if times_gen else float("nan")

@@ -114,6 +114,7 @@ class LutLinear(nn.Module):
         self.register_buffer("alpha", a)
         # kept as a plain attribute like the reference (quant.py:28)
         self.bias = bias
+        self.adapters = None           # an adapters.AdapterBank beside this layer, see forward
         self.reuse_output = False      # see _output
         self._pow2_cache = None        # see _alphas_are_powers_of_two
         self._bias_cache = None        # see _bias_vector
@@ -171,7 +172,12 @@ class LutLinear(nn.Module):
             buf = self._out_cache[(rows, device)] = torch.empty((rows, self.N), dtype=torch.float16, device=device)
         return buf
 
-    def forward(self, x):
+    def forward(self, x, adapter_ids=None):
+        """W_q x + bias; with `adapter_ids` (int32, one per row of x) plus, row by row, the product of the adapter of `self.adapters` that
+        the id names (none where it is not one of them).  Then x is rounded to fp16 first, and the sum is formed in fp16 rows:
+        the layer's result and the adapter's are each rounded once."""
+        if adapter_ids is not None:
+            return self._adapted(x, adapter_ids)
         # (at one row the host bounds the layer: what can be checked natively is)
         K = self.K
         buffers = self._buffers
@@ -187,6 +193,17 @@ class LutLinear(nn.Module):
             bias = self._bias_vector(x.device)
         out = self._output(x.numel() // K, x.device) if self.reuse_output else None
         return native.lutgemm.linear_forward(x, signs, alpha, bias, out, fmt, self.N, K, self.wbit, self.num_groups, pow2)
+
+    def _adapted(self, x, adapter_ids):
+        bank = self.adapters
+        if bank is None:
+            raise ValueError("adapter_ids given, but the layer has no adapters")
+        if bank.K != self.K or bank.N != self.N:
+            raise ValueError(f"adapters of a {bank.K} -> {bank.N} projection beside a {self.K} -> {self.N} layer")
+        half = x if x.dtype is torch.float16 else x.to(torch.float16)
+        y = LutLinear.forward(self, half)
+        y = bank(half, adapter_ids.reshape(-1).to(torch.int32), y, y)
+        return y if x.dtype is torch.float16 else y.to(x.dtype)
 
     def extra_repr(self):
         return "in_features={}, out_features={}, bias={}, wbit={}, group_size={}, alpha_format={}".format(

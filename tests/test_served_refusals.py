@@ -198,3 +198,43 @@ def test_values_follow_the_stated_layout():
         code = bits(words[b, 160 * G + (quad * 16 + d % 16) * 2 * G + d // 16], e)
         scale, low = half[b, 576 * G + g * 64 + quad * 8 + e].float(), half[b, 576 * G + g * 64 + 32 + quad * 8 + e].float()
         assert v[p, 0, d] == (low + scale * code).half()
+
+
+def test_decoder_refuses():
+    from shiftaddllm_amd import decode
+    cfg = decode.DecoderConfig(vocab_size=32, hidden=128, intermediate=128, layers=1, heads=2, kv_heads=1, max_positions=8)
+    make = lambda **kw: decode.LutDecoder(cfg, None, device="cpu", **kw)
+    for kw in (dict(kv_bits=8), dict(kv_bits=4, glue="torch"), dict(kv_bits=4, chain=True), dict(adapters=(2, 8), chain=True), dict(adapters=(2, 0))):
+        with pytest.raises(ValueError):
+            make(**kw)
+    with pytest.raises(ValueError):       # heads of 48 numbers
+        decode.LutDecoder(decode.DecoderConfig(vocab_size=32, hidden=96, intermediate=128, layers=1, heads=2, kv_heads=1, max_positions=8, group_size=32),
+                          None, device="cpu", kv_bits=4)
+    plain, q4 = make(), make(kv_bits=4, batch=2)
+    ids = torch.zeros((1, 2), dtype=torch.long)
+    with pytest.raises(ValueError):
+        plain.prefill(ids)
+    with pytest.raises(ValueError):
+        plain.forward_token(ids[:, 0], [0])
+    for position in ([0], [0, 8], [0, 1, 2]):
+        with pytest.raises(ValueError):
+            q4.forward_token(torch.zeros(2, dtype=torch.long), position)
+    two = torch.zeros((2, 4), dtype=torch.long)
+    for kw in (dict(lengths=[4]), dict(lengths=[5, 1]), dict(lengths=[4, -1]), dict(starts=[5, 0]), dict(starts=[-1, 0]), dict(starts=[0])):
+        with pytest.raises(ValueError):
+            q4.prefill(two, **kw)
+    with pytest.raises(ValueError):
+        q4.prefill(ids)
+    assert hasattr(plain, "k_cache") and not hasattr(q4, "k_cache") and q4.q4[0].data.shape == (2, 1, 1, 40 * 64)
+
+
+def test_linear_layers_keep_their_state():
+    """A layer without adapters has the state it had; with them, the bank's buffers beside its own."""
+    from shiftaddllm_amd.lut_gemm.adapters import AdapterBank
+    from shiftaddllm_amd.lut_gemm.quant import LutLinear
+    lin = LutLinear(64, 32, group_size=32)
+    assert sorted(lin.state_dict()) == ["alpha", "binaryWeight"] and lin.adapters is None
+    with pytest.raises(ValueError):
+        lin(torch.zeros((1, 64)), torch.zeros(1, dtype=torch.int32))
+    lin.adapters = AdapterBank(64, 32, 8, 2)
+    assert sorted(lin.state_dict()) == ["adapters.down", "adapters.scale", "adapters.up", "alpha", "binaryWeight"]
