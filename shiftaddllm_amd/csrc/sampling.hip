@@ -3,9 +3,8 @@
 // Mathematics.  The order is larger logits first, equal ones by index, and every filter keeps a first part of it: the row's
 // tokens are never sorted, only the element is looked for at which a running count or a running sum of weights reaches a target.  The
 // weights, exp((l - m) / temperature) in 64 bits, are held as whole numbers of 2^-bits, so that sums do not depend on the order in
-// which threads add; as many bits as leave room for the sum of a vocabulary, 43 (2^20 tokens) to 51.  A histogram of counts and sums over 4096 equal steps of the logit
-// below the largest, as far as weights reach, says in which step a target is reached; the few tokens of that step are then looked
-// at one by one.  Where they are many (equal logits, an endless temperature) digits of the logit's bits are followed instead.
+// which threads add; as many bits as leave room for the sum of a vocabulary, 43 (2^20 tokens) to 51.  A histogram of sums over steps of
+// a 64th of a power of two says in which step a target is reached; the few tokens of that step are then looked at one by one.  Where they are many (equal logits, an endless temperature) digits of the logit's bits are followed instead.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -21,7 +20,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kSteps = 4096;          // of the histogram
+constexpr int kSteps = 4096;          // of the histogram, 64 to a power of two (52 powers at most)
+constexpr int kCounted = 256;         // top_k from which tokens are counted in the first pass
 constexpr int kPerThread = kSteps / kThreads;
 constexpr int kNear = 4096;           // tokens near the largest that are kept by themselves, at most
 constexpr int kMembers = 1024;        // tokens of a step that are looked at one by one, at most
@@ -36,9 +36,8 @@ struct RowWork {
     u64 sum[kSteps];
     u64 near_[kNear];
     uint32_t count[kSteps];
-    u64 min_sum;
-    uint32_t near_count, unused;
-    float most[kParts], total[kParts], number[kParts];   // of the parts
+    uint32_t near_count, unused[3];
+    float most[kParts], total[kParts], square[kParts], number[kParts];   // of the parts
 };
 
 struct Args {
@@ -47,7 +46,7 @@ struct Args {
     int rows, vocab;
     int bits;           // a weight of 1 is 2^bits
     int parts;          // workgroups that share a row
-    float near_share;   // of the distance from the mean to the largest logit, within which tokens are kept by themselves
+    float near_share, near_spread;   // which tokens are kept by themselves, see scale_of
     const float *temperature;
     const int32_t *top_k;
     const float *top_p, *min_p, *uniform;
@@ -93,22 +92,24 @@ struct Scale {
     float most;        // the largest logit
     double inverse;    // 1 / temperature
     double fractions;  // 256 log2(e) / temperature
-    float steps;       // steps of the histogram per unit of the logit
     int bits;
     int near_steps;    // tokens of earlier steps are kept by themselves
 
-    // The weight as a whole number of 2^-bits; false, and no number, where it is less than half of 2^-bits.  256 log2(e) (l - most) / t = n + f
+    // 256 log2(e) (l - most) / t
+    __device__ __forceinline__ double place(float l) const { return ((double)l - (double)most) * fractions; }
+    // The weight as a whole number of 2^-bits, and the step; false, and neither, where it is less than half of 2^-bits.  The place is n + f
     // with |f| <= 1/2; 2^(n / 256) by powers of two and a table, 2^(f / 256) by its series: terms to f^4, off by 2^-54.  Conversions,
     // roundings and scalings of 64-bit numbers take four times as long as sums and products here, so whole numbers are made by adding
     // 1.5 * 2^52 (2^52), whose last place is one, and powers of two by adding to the exponent.  (With such instructions and a series of
     // twelve terms 256 rows of 131072 logits took 187 us.)  NaN has no weight.  (An infinite `most`: it alone has weight.)
-    __device__ __forceinline__ bool weight(float l, const double *table, u64 &w) const
+    __device__ __forceinline__ bool weight(float l, const double *table, u64 &w, int &step) const
     {
         if (most == INFINITY) {
             w = 1ull << bits;
+            step = 0;
             return l == most;
         }
-        const double y = ((double)l - (double)most) * fractions;
+        const double y = place(l);
         const double shifted = y + 0x1.8p52;
         const int n = (int)(uint32_t)__builtin_bit_cast(u64, shifted);
         const double f = y - (shifted - 0x1.8p52);
@@ -120,11 +121,15 @@ struct Scale {
         const double v = __builtin_fma(p * f, power, power);
         const u64 scaled = __builtin_bit_cast(u64, v) + ((u64)(uint32_t)((n >> 8) + bits) << 52);
         w = __builtin_bit_cast(u64, __builtin_bit_cast(double, scaled) + 0x1p52) & ((1ull << 52) - 1);
+        step = -n >> 2;   // (larger logits in earlier ones)
         return y >= -(double)(kFractions * (bits + 1));
     }
-    // The step: larger logits in earlier ones.  (An infinite `most`: all that has weight is in one.)
-    __device__ __forceinline__ float place(float l) const { return (most - l) * steps; }
-    __device__ __forceinline__ int step(float l) const { return (int)fminf(place(l), (float)(kSteps - 1)); }
+    // Whether a logit is of a step, but for its last hundredth on either side (a difference's place in fp32 is off by 2^-22 of itself).
+    __device__ __forceinline__ bool near_step(float l, int step) const
+    {
+        const float p = (most - l) * (float)(fractions * 0.25);
+        return !(p < (float)step - 0.135f) && (!(p > (float)step + 0.885f) || fractions >= 1e30);
+    }
     __device__ __forceinline__ double exponent(float l) const { return l == most ? 0.0 : ((double)l - (double)most) * inverse; }
 };
 
@@ -132,6 +137,11 @@ struct Scale {
 struct Found {
     uint32_t key, index;
     u64 sum;
+};
+
+// A thread's four steps of the histogram: the sum of all steps before them, and the sums up to each.
+struct Running {
+    u64 before, upto[kPerThread];
 };
 
 struct Shared {
@@ -142,13 +152,13 @@ struct Shared {
     double table[kFractions];                      // 2^(i / 256)
     u64 wave_sum[kWaves];
     uint32_t wave_count[kWaves];
-    float wave_most[kWaves], wave_total[kWaves], wave_number[kWaves];
+    float wave_most[kWaves], wave_total[kWaves], wave_square[kWaves], wave_number[kWaves];
     u64 digit_sum[256];
     uint32_t digit_count[256];
     int step;
     uint32_t members, near_count;
     Found found;
-    u64 before_sum, min_sum;
+    u64 before_sum, total, least_sum;
     uint32_t before_count, digit;
 };
 
@@ -266,148 +276,53 @@ __device__ __forceinline__ N wave_scan(N v)
     return v;
 }
 
-// Sums of (count, sum) over the threads before this one.
-__device__ void exclusive_scan(Shared &s, uint32_t &count, u64 &sum)
+// Sums over the threads before this one; returns the sum of all.
+template <typename N>
+__device__ N exclusive_scan(Shared &s, N &value)
 {
+    N *waves = sizeof(N) == 8 ? (N *)s.wave_sum : (N *)s.wave_count;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t c = wave_scan(count);
-    const u64 w = wave_scan(sum);
+    const N v = wave_scan(value);
     __syncthreads();
-    if (lane == 63) {
-        s.wave_count[wave] = c;
-        s.wave_sum[wave] = w;
-    }
+    if (lane == 63) waves[wave] = v;
     __syncthreads();
-    count = c - count;
-    sum = w - sum;
+    value = v - value;
+    N all = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-        count += i < wave ? s.wave_count[i] : 0;
-        sum += i < wave ? s.wave_sum[i] : 0;
+        const N its = waves[i];
+        value += i < wave ? its : 0;
+        all += its;
     }
+    return all;
 }
 
-// The first element of the order at which the running count is at least `count` (by_sum false) or the running sum at least `sum`;
-// the row holds one.
-template <typename R>
-__device__ Found reach(Shared &s, const R &row, const Scale &scale, bool by_sum, uint32_t count, u64 sum)
+// What is rarely called for stands in functions of its own: the kernel's instructions are all fetched anew for every row.
+
+// Counts by steps (where they are not there yet) and the sum of weights of at least `least`, over all of a row.
+template <typename T>
+__device__ __noinline__ void count_row(Shared *s, const Row<T> row, const Scale scale, bool count, u64 least)
 {
-    const int tid = threadIdx.x;
-    __syncthreads();
-    // the step (the arrays hold running totals)
-    for (int i = 0; i < kPerThread; ++i) {
-        const int b = i * kThreads + tid;
-        const uint32_t c0 = !by_sum && b > 0 ? s.count[b - 1] : 0;
-        const u64 w0 = b > 0 ? s.sum[b - 1] : 0;
-        if (by_sum ? w0 < sum && s.sum[b] >= sum : c0 < count && s.count[b] >= count) {
-            s.step = b;
-            s.before_count = c0;
-            s.before_sum = w0;
-        }
-    }
-    if (tid == 0) s.members = 0;
-    __syncthreads();
-    const int step = s.step;
-    uint32_t before_count = s.before_count;
-    u64 before_sum = s.before_sum;
-    auto gather = [&](float l, uint32_t i) {
+    u64 sum = 0;
+    row.for_each([&](float l, uint32_t) {
         u64 w;
-        if (!scale.weight(l, s.table, w) || scale.step(l) != step) return;
-        const uint32_t at = atomicAdd(&s.members, 1u);
-        if (at >= (uint32_t)kMembers) return;
-        s.member[at] = (u64)key_of(l) << 32 | (uint32_t)~i;
-        s.member_weight[at] = w;
-    };
-    if (step < scale.near_steps && s.near_count <= (uint32_t)kNear)
-        for (uint32_t i = tid; i < s.near_count; i += kThreads) gather(logit_of_key((uint32_t)(s.near_[i] >> 32)), (uint32_t)~s.near_[i]);
-    else row.by_pieces([&](const float (&l)[R::kPiece], int i) {
-        // (most pieces hold none: one branch for all of a piece's logits.  The last step holds what lies behind it too, and what an
-        // infinite logit's distance is no number for)
-        bool any = false;
-        const float from = (float)step, past = step == kSteps - 1 ? INFINITY : from + 1.0f;
-#pragma unroll
-        for (int e = 0; e < R::kPiece; ++e) {
-            const float place = scale.place(l[e]);
-            any |= place >= from && place < past;
-        }
-        if (!any && step < kSteps - 1) return;
-#pragma unroll
-        for (int e = 0; e < R::kPiece; ++e) gather(l[e], (uint32_t)(i + e));
+        int step;
+        if (!scale.weight(l, s->table, w, step)) return;
+        if (count) atomicAdd(&s->count[step], 1u);
+        sum += w >= least ? w : 0;
     });
-    __syncthreads();
-    const uint32_t members = s.members;
-    if (members <= (uint32_t)kMembers) {
-        u64 mine = 0, own = 0;
-        int part = -1;
-        if (tid < (int)members) {
-            mine = s.member[tid];
-            own = s.member_weight[tid];
-            part = min((int)((scale.place(logit_of_key((uint32_t)(mine >> 32))) - (float)step) * 256.0f), 255);
-        }
-        uint32_t rivals = members;
-        if (members > 64) {   // a 256th of the step first: each of its members is held against the others
-            if (tid < 256) {
-                s.digit_count[tid] = 0;
-                s.digit_sum[tid] = 0;
-            }
-            __syncthreads();
-            if (part >= 0) {
-                atomicAdd(&s.digit_count[part], 1u);
-                atomicAdd(&s.digit_sum[part], own);
-            }
-            if (tid == 0) s.members = 0;
-            __syncthreads();
-            if (tid < 64) {
-                uint32_t c[4];
-                u64 w[4];
-                uint32_t all_c = 0;
-                u64 all_w = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    c[i] = s.digit_count[4 * tid + i];
-                    w[i] = s.digit_sum[4 * tid + i];
-                    all_c += c[i];
-                    all_w += w[i];
-                }
-                uint32_t at_c = before_count + wave_scan(all_c) - all_c;
-                u64 at_w = before_sum + wave_scan(all_w) - all_w;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (by_sum ? at_w < sum && at_w + w[i] >= sum : at_c < count && at_c + c[i] >= count) {
-                        s.digit = 4 * tid + i;
-                        s.before_count = at_c;
-                        s.before_sum = at_w;
-                    }
-                    at_c += c[i];
-                    at_w += w[i];
-                }
-            }
-            __syncthreads();
-            before_count = s.before_count;
-            before_sum = s.before_sum;
-            if (part != (int)s.digit) part = -1;
-            if (part >= 0) {
-                const uint32_t at = atomicAdd(&s.members, 1u);
-                s.member[at] = mine;
-                s.member_weight[at] = own;
-            }
-            __syncthreads();
-            rivals = s.members;
-        }
-        if (part >= 0) {
-            uint32_t c = before_count + 1;
-            u64 w = before_sum + own;
-            for (uint32_t j = 0; j < rivals; ++j) {
-                const bool ahead = s.member[j] > mine;
-                c += ahead;
-                w += ahead ? s.member_weight[j] : 0;
-            }
-            if (by_sum ? w >= sum && w - own < sum : c == count) s.found = {(uint32_t)(mine >> 32), (uint32_t)~mine, w};
-        }
-        __syncthreads();
-        return s.found;
-    }
-    // many: the key's digits of eight bits, from the top
+    sum = wave_scan(sum);
+    if ((threadIdx.x & 63) == 63 && sum) atomicAdd(&s->least_sum, sum);
+}
+
+// The element of a step at which a target is reached where the step has too many to be held against each other: by the digits, of eight bits,
+// of the key, then by index.
+template <typename T>
+__device__ __noinline__ void reach_by_digits(Shared *sp, const Row<T> row, const Scale scale, int step, uint32_t before_count, u64 before_sum, bool by_sum,
+                                             uint32_t count, u64 sum)
+{
+    Shared &s = *sp;
+    const int tid = threadIdx.x;
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
@@ -419,7 +334,8 @@ __device__ Found reach(Shared &s, const R &row, const Scale &scale, bool by_sum,
         row.for_each([&](float l, uint32_t) {
             const uint32_t key = key_of(l);
             u64 w;
-            if (!scale.weight(l, s.table, w) || scale.step(l) != step || (shift < 24 && key >> (shift + 8) != prefix)) return;
+            int its;
+            if (!scale.weight(l, s.table, w, its) || its != step || (shift < 24 && key >> (shift + 8) != prefix)) return;
             atomicAdd(&s.digit_count[(key >> shift) & 255u], 1u);
             atomicAdd(&s.digit_sum[(key >> shift) & 255u], w);
         });
@@ -442,18 +358,146 @@ __device__ Found reach(Shared &s, const R &row, const Scale &scale, bool by_sum,
     }
     // equal logits: the one so many places further on
     u64 w;
-    scale.weight(logit_of_key(prefix), s.table, w);
+    int unused;
+    scale.weight(logit_of_key(prefix), s.table, w, unused);
     const uint32_t place = by_sum ? (uint32_t)((sum - before_sum + w - 1) / w) : count - before_count;   // 1 for the first
     const int own = (row.vocab + kThreads - 1) / kThreads, first = min(tid * own, row.vocab), past = min(first + own, row.vocab);
     uint32_t c = 0;
     for (int i = first; i < past; ++i) c += key_of(row.at(i)) == prefix;
     uint32_t ahead = c;
-    u64 unused = 0;
-    exclusive_scan(s, ahead, unused);
+    exclusive_scan(s, ahead);
     if (ahead < place && ahead + c >= place) {
         uint32_t at = ahead;
         for (int i = first; i < past; ++i)
             if (key_of(row.at(i)) == prefix && ++at == place) s.found = {prefix, (uint32_t)i, before_sum + place * w};
+    }
+    __syncthreads();
+}
+
+// The first element of the order at which the running count is at least `count` (by_sum false; s.count holds the steps' counts) or the
+// running sum at least `sum`; the row holds one.
+template <typename T>
+__device__ __forceinline__ Found reach(Shared &s, const Row<T> &row, const Scale &scale, const Running &run, bool by_sum, uint32_t count, u64 sum)
+{
+    const int tid = threadIdx.x;
+    if (by_sum) {
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            const u64 w0 = i > 0 ? run.upto[i - 1] : run.before;
+            if (w0 < sum && run.upto[i] >= sum) {
+                s.step = tid * kPerThread + i;
+                s.before_count = 0;
+                s.before_sum = w0;
+            }
+        }
+    } else {
+        uint32_t c[kPerThread], all = 0;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) all += c[i] = s.count[tid * kPerThread + i];
+        uint32_t c0 = all;
+        exclusive_scan(s, c0);
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            if (c0 < count && c0 + c[i] >= count) {
+                s.step = tid * kPerThread + i;
+                s.before_count = c0;
+                s.before_sum = i > 0 ? run.upto[i - 1] : run.before;
+            }
+            c0 += c[i];
+        }
+    }
+    if (tid == 0) s.members = 0;
+    __syncthreads();
+    const int step = s.step;
+    uint32_t before_count = s.before_count;
+    u64 before_sum = s.before_sum;
+    auto candidate = [&](u64 entry) {
+        const uint32_t at = atomicAdd(&s.members, 1u);
+        if (at < (uint32_t)kMembers) s.member[at] = entry;
+    };
+    if (step < scale.near_steps && s.near_count <= (uint32_t)kNear)
+        for (uint32_t i = tid; i < s.near_count; i += kThreads) {
+            const u64 entry = s.near_[i];
+            if (scale.near_step(logit_of_key((uint32_t)(entry >> 32)), step)) candidate(entry);
+        }
+    else row.by_pieces([&](const float (&l)[Row<T>::kPiece], int i) {
+#pragma unroll
+        for (int e = 0; e < Row<T>::kPiece; ++e)
+            if (scale.near_step(l[e], step)) candidate((u64)key_of(l[e]) << 32 | (uint32_t)~(uint32_t)(i + e));
+    });
+    __syncthreads();
+    const uint32_t candidates = s.members;
+    if (candidates > (uint32_t)kMembers) {
+        reach_by_digits(&s, row, scale, step, before_count, before_sum, by_sum, count, sum);
+        return s.found;
+    }
+    // A candidate a thread: its weight, and the 256th of the step that it is in (-1: it is of another step).
+    u64 mine = 0, own = 0;
+    int part = -1;
+    if (tid < (int)candidates) {
+        mine = s.member[tid];
+        const float l = logit_of_key((uint32_t)(mine >> 32));
+        int its;
+        // (the step's places lie between 4 * step - 2 and 4 * step + 6 below 0; an infinite logit's is none)
+        if (scale.weight(l, s.table, own, its) && its == step)
+            part = min(max((int)(((scale.most == INFINITY ? 0.0 : -scale.place(l)) - (4 * step - 2)) * 32.0), 0), 255);
+    }
+    const bool many = candidates > 64;   // a 256th of the step first: each of its members is held against the others
+    if (many && tid < 256) {
+        s.digit_count[tid] = 0;
+        s.digit_sum[tid] = 0;
+    }
+    __syncthreads();
+    if (many) {
+        if (part >= 0) {
+            atomicAdd(&s.digit_count[part], 1u);
+            atomicAdd(&s.digit_sum[part], own);
+        }
+        __syncthreads();
+        if (tid < 64) {
+            uint32_t c[4], all_c = 0;
+            u64 w[4], all_w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                all_c += c[i] = s.digit_count[4 * tid + i];
+                all_w += w[i] = s.digit_sum[4 * tid + i];
+            }
+            uint32_t at_c = before_count + wave_scan(all_c) - all_c;
+            u64 at_w = before_sum + wave_scan(all_w) - all_w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (by_sum ? at_w < sum && at_w + w[i] >= sum : at_c < count && at_c + c[i] >= count) {
+                    s.digit = 4 * tid + i;
+                    s.before_count = at_c;
+                    s.before_sum = at_w;
+                }
+                at_c += c[i];
+                at_w += w[i];
+            }
+        }
+        __syncthreads();
+        before_count = s.before_count;
+        before_sum = s.before_sum;
+        if (part != (int)s.digit) part = -1;
+    }
+    if (tid == 0) s.members = 0;
+    __syncthreads();
+    if (part >= 0) {
+        const uint32_t at = atomicAdd(&s.members, 1u);
+        s.member[at] = mine;
+        s.member_weight[at] = own;
+    }
+    __syncthreads();
+    const uint32_t rivals = s.members;
+    if (part >= 0) {
+        uint32_t c = before_count + 1;
+        u64 w = before_sum + own;
+        for (uint32_t j = 0; j < rivals; ++j) {
+            const bool ahead = s.member[j] > mine;
+            c += ahead;
+            w += ahead ? s.member_weight[j] : 0;
+        }
+        if (by_sum ? w >= sum && w - own < sum : c == count) s.found = {(uint32_t)(mine >> 32), (uint32_t)~mine, w};
     }
     __syncthreads();
     return s.found;
@@ -475,17 +519,26 @@ struct Asked {
     }
 };
 
-// `mean`: of the logits that are finite.  (A greedy row: its weights are of no account, the first of its largest logits is.  An
-// endless temperature: all that is not -inf weighs the same.)
-__device__ __forceinline__ Scale scale_of(const Args &a, const Asked &ask, float most, float mean)
+// Some of a row's logits: the largest of all, and sums, of them and of their squares, and number of those looked at.
+struct Survey {
+    float most, total, square, number;
+};
+
+// Tokens near the largest logit are kept by themselves, so that a target that is reached among them needs no further look at the row.  They are
+// those within a share of the distance from the mean to the largest, or so many standard deviations above the mean, whichever takes in
+// more: some 1500 of normally distributed logits, whether or not others stand far above them.  (Rows with more of them than there is
+// room for are looked at again instead, which costs time only.)  A greedy row: its weights are of no account, the first of its largest
+// logits is.  An endless temperature: all that is not -inf weighs the same.
+__device__ __forceinline__ Scale scale_of(const Args &a, const Asked &ask, const Survey &v)
 {
     Scale s;
-    s.most = most;
+    s.most = v.most;
     s.inverse = ask.greedy ? 1e30 : ask.t == INFINITY ? 1e-300 : 1.0 / (double)ask.t;
     s.fractions = s.inverse * (kFractions * 1.4426950408889634);
-    s.steps = ask.greedy ? 1e30f : fminf((float)kSteps / ((a.bits + 1) * 0.6931472f) / ask.t, 1e30f);
     s.bits = a.bits;
-    const float near_ = (most - mean) * a.near_share * s.steps;
+    const float mean = v.total / v.number, spread = sqrtf(fmaxf(v.square / v.number - mean * mean, 0.0f));
+    const float reach = fmaxf((v.most - mean) * a.near_share, v.most - mean - a.near_spread * spread);
+    const float near_ = reach * (float)fmin(s.fractions * 0.25, 1e30);
     s.near_steps = near_ < (float)kSteps ? (int)near_ + 1 : kSteps;
     return s;
 }
@@ -527,18 +580,18 @@ __device__ __forceinline__ float largest_of(const u32x4 &raw)
     }
 }
 
-// The largest logit of (a part of) a row, and sum and number of the finite ones among the first of every piece.
+// The largest logit of (a part of) a row, and sums and number of the finite ones among the first of every piece.
 template <typename T>
-__device__ void survey(Shared &s, const Row<T> &row, float &most, float &total, float &number)
+__device__ Survey survey(Shared &s, const Row<T> &row)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    most = -INFINITY;
-    total = number = 0.0f;
+    float most = -INFINITY, total = 0.0f, square = 0.0f, number = 0.0f;
     row.raw_pieces([&](int piece, const u32x4 &raw, bool inside) {
         if (inside) {
             const float first = logit_of(*(const T *)&raw);
             most = fmaxf(most, largest_of<T>(raw));
             total += fabsf(first) < INFINITY ? first : 0.0f;
+            square += fabsf(first) < INFINITY ? first * first : 0.0f;
             number += fabsf(first) < INFINITY ? 1.0f : 0.0f;
         } else {
             row.visit(piece, raw, false, [&](const float (&l)[Row<T>::kPiece], int) {
@@ -549,20 +602,24 @@ __device__ void survey(Shared &s, const Row<T> &row, float &most, float &total, 
     });
     most = over_wave(most, [](float x, float y) { return fmaxf(x, y); });
     total = over_wave(total, [](float x, float y) { return x + y; });
+    square = over_wave(square, [](float x, float y) { return x + y; });
     number = over_wave(number, [](float x, float y) { return x + y; });
     if (lane == 0) {
         s.wave_most[wave] = most;
         s.wave_total[wave] = total;
+        s.wave_square[wave] = square;
         s.wave_number[wave] = number;
     }
     __syncthreads();
-    total = number = 0.0f;
+    Survey v = {most, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        most = fmaxf(most, s.wave_most[w]);
-        total += s.wave_total[w];
-        number += s.wave_number[w];
+        v.most = fmaxf(v.most, s.wave_most[w]);
+        v.total += s.wave_total[w];
+        v.square += s.wave_square[w];
+        v.number += s.wave_number[w];
     }
+    return v;
 }
 
 __device__ void clear(Shared &s)
@@ -573,39 +630,35 @@ __device__ void clear(Shared &s)
     }
     if (threadIdx.x < kFractions) s.table[threadIdx.x] = kTable.power[threadIdx.x];
     if (threadIdx.x == 0) {
-        s.min_sum = 0;
+        s.least_sum = 0;
         s.near_count = 0;
     }
 }
 
-// Counts and sums by steps, the tokens near the largest, and the sum of what min_p leaves, of (a part of) a row.
+// Sums by steps and the tokens near the largest, of (a part of) a row; counts too where many are asked for.
 template <typename T>
 __device__ void histogram(Shared &s, const Row<T> &row, const Scale &scale, const Asked &ask)
 {
-    u64 min_sum = 0;
-    const u64 min_weight = (u64)__builtin_ceil((double)ask.least * (double)(1ull << scale.bits));
     row.by_pieces([&](const float (&l)[Row<T>::kPiece], int i) {
         u64 w[Row<T>::kPiece];
+        int step[Row<T>::kPiece];
         bool live[Row<T>::kPiece];
 #pragma unroll
         for (int e = 0; e < Row<T>::kPiece; ++e) {
-            live[e] = scale.weight(l[e], s.table, w[e]);
+            live[e] = scale.weight(l[e], s.table, w[e], step[e]);
             asm volatile("" : "+v"(w[e]));   // (formed side by side, not each behind a branch of its own)
         }
 #pragma unroll
         for (int e = 0; e < Row<T>::kPiece; ++e) {
             if (!live[e]) continue;
-            const int b = scale.step(l[e]);
-            if (ask.k > 0) atomicAdd(&s.count[b], 1u);   // (counts are asked for by top_k only: the ends of other parts are compared by their sums)
-            atomicAdd(&s.sum[b], w[e]);
-            if (ask.least > 0.0f) min_sum += w[e] >= min_weight ? w[e] : 0;
-            if (b < scale.near_steps) {
+            atomicAdd(&s.sum[step[e]], w[e]);
+            if (ask.k >= kCounted) atomicAdd(&s.count[step[e]], 1u);
+            if (step[e] < scale.near_steps) {
                 const uint32_t at = atomicAdd(&s.near_count, 1u);
                 if (at < (uint32_t)kNear) s.near_[at] = (u64)key_of(l[e]) << 32 | (uint32_t)~(uint32_t)(i + e);
             }
         }
     });
-    if (ask.least > 0.0f) atomicAdd(&s.min_sum, min_sum);
 }
 
 // The token, from the histogram of the whole row.
@@ -614,36 +667,64 @@ __device__ void choose(const Args &a, Shared &s, const Row<T> &row, const Scale 
 {
     const int tid = threadIdx.x;
     __syncthreads();
+    Running run;
+    u64 total;
     {   // running totals
-        uint32_t c = 0;
-        u64 w = 0;
+        u64 w[kPerThread], all = 0;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            c += s.count[tid * kPerThread + i];
-            w += s.sum[tid * kPerThread + i];
+        for (int i = 0; i < kPerThread; ++i) all += w[i] = s.sum[tid * kPerThread + i];
+        run.before = all;
+        total = exclusive_scan(s, run.before);
+        u64 upto = run.before;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) run.upto[i] = upto += w[i];
+    }
+    const bool by_count = ask.k > 0 && ask.k < row.vocab, by_least = ask.least > 0.0f;
+    uint32_t counted = 0;
+    if (by_count || by_least) {
+        // Counts and the sum of what min_p leaves, from the tokens near the largest unless very many are asked for.
+        const u64 least = by_least ? min((u64)__builtin_ceil((double)ask.least * (double)(1ull << scale.bits)), 1ull << scale.bits) : ~0ull;
+        const bool kept = s.near_count <= (uint32_t)kNear, count = by_count && ask.k < kCounted;
+        if (kept && (!count || s.near_count >= (uint32_t)ask.k) && (!by_least || -64.0f * log2f(ask.least) + 2.0f < (float)scale.near_steps)) {
+            u64 sum = 0;
+            for (uint32_t i = tid; i < s.near_count; i += kThreads) {
+                u64 w;
+                int step;
+                if (!scale.weight(logit_of_key((uint32_t)(s.near_[i] >> 32)), s.table, w, step)) continue;
+                if (count) atomicAdd(&s.count[step], 1u);
+                sum += w >= least ? w : 0;
+            }
+            sum = wave_scan(sum);
+            if ((tid & 63) == 63 && sum) atomicAdd(&s.least_sum, sum);
+        } else {
+            count_row(&s, row, scale, count, least);
         }
-        exclusive_scan(s, c, w);
+        __syncthreads();
+        if (by_count) {
+            uint32_t some = 0;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-            c += s.count[tid * kPerThread + i];
-            w += s.sum[tid * kPerThread + i];
-            s.count[tid * kPerThread + i] = c;
-            s.sum[tid * kPerThread + i] = w;
+            for (int i = 0; i < kPerThread; ++i) some += s.count[tid * kPerThread + i];
+            counted = exclusive_scan(s, some);
         }
     }
-    __syncthreads();
-    u64 total = s.sum[kSteps - 1];
-    if (ask.k > 0 && (uint32_t)ask.k < s.count[kSteps - 1]) total = reach(s, row, scale, false, (uint32_t)ask.k, 0).sum;
-    if (ask.p < 1.0f) {
-        const double target = __builtin_ceil((double)fmaxf(ask.p, 0.0f) * (double)total);
-        total = min(total, reach(s, row, scale, true, 0, target < 1.0 ? 1 : (u64)target).sum);
-    }
-    if (ask.least > 0.0f) total = min(total, s.min_sum);
     float u = a.uniform[r];
     u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-    u64 target = (u64)__builtin_floor((double)u * (double)total);
-    if (target >= total) target = total - 1;
-    const Found f = reach(s, row, scale, true, 0, target + 1);
+    Found f;
+    // The ends of what top_k and top_p leave, then the token.
+#pragma nounroll
+    for (int turn = by_count && (uint32_t)ask.k <= counted ? 0 : 1; turn < 3; ++turn) {
+        u64 target = 0;
+        if (turn == 1) {
+            if (!(ask.p < 1.0f)) continue;
+            const double part = __builtin_ceil((double)fmaxf(ask.p, 0.0f) * (double)total);
+            target = part < 1.0 ? 1 : (u64)part;
+        } else if (turn == 2) {
+            if (by_least) total = min(total, s.least_sum);
+            target = min((u64)__builtin_floor((double)u * (double)total), total - 1) + 1;
+        }
+        f = reach(s, row, scale, run, turn > 0, (uint32_t)ask.k, target);
+        if (turn < 2) total = min(total, f.sum);
+    }
     if (tid == 0) {
         a.ids[r] = f.index;
         if (a.logprob) a.logprob[r] = ask.greedy ? 0.0f : (float)(scale.exponent(logit_of_key(f.key)) - log((double)total / (double)(1ull << a.bits)));
@@ -666,10 +747,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Args a)
     const Row<T> row((const T *)a.logits + r * a.row_stride, a.vocab, 0, 1);
     const Asked ask(a, r);
     clear(s);
-    float most, total, number;
-    survey(s, row, most, total, number);
-    if (most == -INFINITY) return nothing(a, r);
-    const Scale scale = scale_of(a, ask, most, total / number);
+    const Survey v = survey(s, row);
+    if (v.most == -INFINITY) return nothing(a, r);
+    const Scale scale = scale_of(a, ask, v);
     histogram(s, row, scale, ask);
     choose(a, s, row, scale, ask, r);
 }
@@ -687,28 +767,26 @@ __global__ void __launch_bounds__(kThreads) survey_kernel(const Args a)
         work.sum[b] = 0;
         work.count[b] = 0;
     }
-    float most, total, number;
-    survey(s, row, most, total, number);
+    const Survey v = survey(s, row);
     if (threadIdx.x != 0) return;
-    work.most[part] = most;
-    work.total[part] = total;
-    work.number[part] = number;
-    if (part == 0) {
-        work.min_sum = 0;
-        work.near_count = 0;
-    }
+    work.most[part] = v.most;
+    work.total[part] = v.total;
+    work.square[part] = v.square;
+    work.number[part] = v.number;
+    if (part == 0) work.near_count = 0;
 }
 
 __device__ __forceinline__ bool scale_of_row(const Args &a, const Asked &ask, const RowWork &work, Scale &scale)
 {
-    float most = -INFINITY, total = 0.0f, number = 0.0f;
+    Survey v = {-INFINITY, 0.0f, 0.0f, 0.0f};
     for (int i = 0; i < a.parts; ++i) {
-        most = fmaxf(most, work.most[i]);
-        total += work.total[i];
-        number += work.number[i];
+        v.most = fmaxf(v.most, work.most[i]);
+        v.total += work.total[i];
+        v.square += work.square[i];
+        v.number += work.number[i];
     }
-    scale = scale_of(a, ask, most, total / number);
-    return most > -INFINITY;
+    scale = scale_of(a, ask, v);
+    return v.most > -INFINITY;
 }
 
 template <typename T>
@@ -734,7 +812,6 @@ __global__ void __launch_bounds__(kThreads) histogram_kernel(const Args a)
     const uint32_t own = s.near_count;
     if (tid == 0) {
         s.members = own ? atomicAdd(&work.near_count, own) : 0;
-        if (s.min_sum) atomicAdd(&work.min_sum, s.min_sum);
     }
     __syncthreads();
     for (uint32_t i = tid; i < own && s.members + i < (uint32_t)kNear && i < (uint32_t)kNear; i += kThreads) work.near_[s.members + i] = s.near_[i];
@@ -760,7 +837,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const Args a)
     if (tid < kFractions) s.table[tid] = kTable.power[tid];
     if (tid == 0) {
         s.near_count = listed;
-        s.min_sum = work.min_sum;
+        s.least_sum = 0;
     }
     choose(a, s, row, scale, ask, r);
 }
@@ -771,11 +848,19 @@ int launch_status()
     return e == hipSuccess ? LUTGEMM_OK : lutgemm_internal_hip_fail((int)e);
 }
 
-// Tokens within this share of the distance from the mean logit to the largest are kept by themselves, so that a target that
-// is reached among them needs no further look at the row: for normally distributed logits some 2000 of them (half the room there is).
+// The share of the distance from the mean to the largest of normally distributed logits above which 1500 of them lie, and the standard
+// deviations above the mean (the normal distribution's quantile, Abramowitz and Stegun 26.2.22).
+float near_spread(int vocab)
+{
+    if (vocab <= kNear) return -1e30f;   // (all of them)
+    const float share = 1500.0f / vocab;
+    const float t = sqrtf(-2.0f * logf(share < 0.5f ? share : 0.5f));
+    return t - (2.30753f + 0.27061f * t) / (1.0f + 0.99229f * t + 0.04481f * t * t);
+}
+
 float near_share(int vocab)
 {
-    return vocab <= 8000 ? 1.0f : 1.0f - sqrtf(logf(vocab / 8000.0f) / logf((float)vocab));
+    return vocab <= kNear ? 1.0f : 1.0f - near_spread(vocab) / sqrtf(2.0f * logf((float)vocab));
 }
 
 // Workgroups that share a row, in three launches instead of one: where rows leave CUs idle and are long enough to pay for the two more
@@ -822,6 +907,7 @@ int lutgemm_sample_tokens(const lutgemm_sampling *c, void *workspace, size_t wor
     a.bits = bits;
     a.parts = parts_of(c->rows, c->vocab);
     a.near_share = near_share(c->vocab);
+    a.near_spread = near_spread(c->vocab);
     a.temperature = c->temperature;
     a.top_k = c->top_k;
     a.top_p = c->top_p;
