@@ -864,14 +864,13 @@ float near_share(int vocab)
 }
 
 // Workgroups that share a row, in three launches instead of one: where rows leave CUs idle and are long enough to pay for the two more
-// launches, and for the addition of histograms, which takes longer the more of them there are.  One row of 131072 logits 64.6 -> 36.4 us with
-// 8 (32 parts 33.1, but 8 rows of 50272 28.9 instead of 26.0), 128 rows 84.6 -> 77.2 with 2, 8 rows of 50272 36.0 -> 30.8; one of 32000 24.4 -> 23.3
-// with 7 without filters, 31.9 -> 30.3 with all, 64 rows of 50272 38.2 -> 37.4 with 4: not worth them.
+// launches and for the addition of histograms, which takes longer the more of them there are.  With all filters, one workgroup against as many as
+// here: one row of 16384 22.2 and 25.8 us, of 32000 28.2 and 26.2; 8 rows of 50272 34.7 and 27.3, 64 35.4 and 32.4; 64 rows of 131072 63.3
+// and 40.3, 128 66.2 and 54.3.
 int parts_of(int rows, int vocab)
 {
-    if (vocab < 40000 || (rows > 32 && vocab < 80000)) return 1;
-    const int parts = 256 / rows;
-    return parts > 8 ? 8 : parts < 1 ? 1 : parts;
+    if (vocab < 28000) return 1;
+    return rows <= 16 ? 8 : rows <= 64 ? 4 : rows <= 128 ? 2 : 1;
 }
 
 bool sizes_fit(int rows, int vocab) { return rows >= 1 && rows <= 65535 && vocab >= 1 && vocab <= 1 << 20; }
