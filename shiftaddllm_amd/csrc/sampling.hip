@@ -90,25 +90,22 @@ __device__ const Table kTable;
 // What a row's weights are formed with.
 struct Scale {
     float most;        // the largest logit
+    double origin;     // the same; 2^128 where it is infinite (then it alone has weight: `fractions` is very large)
     double inverse;    // 1 / temperature
     double fractions;  // 256 log2(e) / temperature
+    double least;      // the place of a weight of 2^-bits / 4
     int bits;
     int near_steps;    // tokens of earlier steps are kept by themselves
 
-    // 256 log2(e) (l - most) / t
-    __device__ __forceinline__ double place(float l) const { return ((double)l - (double)most) * fractions; }
-    // The weight as a whole number of 2^-bits, and the step; false, and neither, where it is less than half of 2^-bits.  The place is n + f
-    // with |f| <= 1/2; 2^(n / 256) by powers of two and a table, 2^(f / 256) by its series: terms to f^4, off by 2^-54.  Conversions,
-    // roundings and scalings of 64-bit numbers take four times as long as sums and products here, so whole numbers are made by adding
-    // 1.5 * 2^52 (2^52), whose last place is one, and powers of two by adding to the exponent.  (With such instructions and a series of
-    // twelve terms 256 rows of 131072 logits took 187 us.)  NaN has no weight.  (An infinite `most`: it alone has weight.)
+    // 256 log2(e) (l - most) / t, not less than `least`, and that for NaN
+    __device__ __forceinline__ double place(float l) const { return fmin(fmax(((double)l - origin) * fractions, least), 0.0); }
+    // The weight as a whole number of 2^-bits, and the step; false where it is less than half of 2^-bits: 0, and a step behind all others.
+    // The place is n + f with |f| <= 1/2; 2^(n / 256) by powers of two and a table, 2^(f / 256) by its series: terms to f^4, off by
+    // 2^-54.  Conversions, roundings and scalings of 64-bit numbers take four times as long as sums and products here, so whole numbers are
+    // made by adding 1.5 * 2^52 (2^52), whose last place is one, and powers of two by adding to the exponent (with such instructions and a
+    // series of twelve terms 256 rows of 131072 logits took 187 us).  No branches: several weights are formed side by side.
     __device__ __forceinline__ bool weight(float l, const double *table, u64 &w, int &step) const
     {
-        if (most == INFINITY) {
-            w = 1ull << bits;
-            step = 0;
-            return l == most;
-        }
         const double y = place(l);
         const double shifted = y + 0x1.8p52;
         const int n = (int)(uint32_t)__builtin_bit_cast(u64, shifted);
@@ -122,7 +119,7 @@ struct Scale {
         const u64 scaled = __builtin_bit_cast(u64, v) + ((u64)(uint32_t)((n >> 8) + bits) << 52);
         w = __builtin_bit_cast(u64, __builtin_bit_cast(double, scaled) + 0x1p52) & ((1ull << 52) - 1);
         step = -n >> 2;   // (larger logits in earlier ones)
-        return y >= -(double)(kFractions * (bits + 1));
+        return w != 0;
     }
     // Whether a logit is of a step, but for its last hundredth on either side (a difference's place in fp32 is off by 2^-22 of itself).
     __device__ __forceinline__ bool near_step(float l, int step) const
@@ -180,7 +177,9 @@ struct Row {
     }
     __device__ __forceinline__ bool whole(int piece) const { return piece * kPiece >= skip && (piece + 1) * kPiece <= skip + vocab; }
     // f(piece, its 16 bytes, whether all of them are the row's): whole pieces, several at a time, then what the row's ends have of theirs.
-    template <typename F>
+    // AHEAD: the next ones are asked for while some are looked at, which pays where that is much work (the histogram's pass; a survey of 128
+    // rows of 131072 takes 15 us so, and 13 without).
+    template <bool AHEAD, typename F>
     __device__ __forceinline__ void raw_pieces(F f) const
     {
         if (begin == past) return;
@@ -189,16 +188,27 @@ struct Row {
         int p0 = from + threadIdx.x, end = threadIdx.x == 0 && from > begin ? begin : threadIdx.x == 1 && to < past && past - 1 > begin ? past - 1 : -1;
         // (a row of one piece that is not whole: the first thread's)
         if (past - 1 == begin && threadIdx.x == 1) end = -1;
+        u32x4 ahead[kAtOnce];
+        auto ask = [&](u32x4 (&into)[kAtOnce]) {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+                if (p0 + u * kThreads < to) into[u] = pieces[p0 + u * kThreads];
+        };
+        if constexpr (AHEAD) ask(ahead);
         while (true) {
             u32x4 raw[kAtOnce];
             int number = 0, base = p0;
             const bool inside = p0 < to;
             if (inside) {
                 number = min((to - p0 + kThreads - 1) / kThreads, kAtOnce);
+                if constexpr (AHEAD) {
 #pragma unroll
-                for (int u = 0; u < kAtOnce; ++u)
-                    if (u < number) raw[u] = pieces[p0 + u * kThreads];
+                    for (int u = 0; u < kAtOnce; ++u) raw[u] = ahead[u];
+                } else {
+                    ask(raw);
+                }
                 p0 += kAtOnce * kThreads;
+                if constexpr (AHEAD) ask(ahead);
             } else if (end >= 0) {
                 T part[kPiece];
 #pragma unroll
@@ -234,15 +244,15 @@ struct Row {
         }
         f(l, i);
     }
-    template <typename F>
+    template <bool AHEAD, typename F>
     __device__ __forceinline__ void by_pieces(F f) const
     {
-        raw_pieces([&](int piece, const u32x4 &raw, bool inside) { visit(piece, raw, inside, f); });
+        raw_pieces<AHEAD>([&](int piece, const u32x4 &raw, bool inside) { visit(piece, raw, inside, f); });
     }
     template <typename F>
     __device__ __forceinline__ void for_each(F f) const
     {
-        by_pieces([&](const float (&l)[kPiece], int i) {
+        by_pieces<false>([&](const float (&l)[kPiece], int i) {
 #pragma unroll
                 for (int e = 0; e < kPiece; ++e) f(l[e], (uint32_t)(i + e));
         });
@@ -420,7 +430,7 @@ __device__ __forceinline__ Found reach(Shared &s, const Row<T> &row, const Scale
             const u64 entry = s.near_[i];
             if (scale.near_step(logit_of_key((uint32_t)(entry >> 32)), step)) candidate(entry);
         }
-    else row.by_pieces([&](const float (&l)[Row<T>::kPiece], int i) {
+    else row.template by_pieces<false>([&](const float (&l)[Row<T>::kPiece], int i) {
 #pragma unroll
         for (int e = 0; e < Row<T>::kPiece; ++e)
             if (scale.near_step(l[e], step)) candidate((u64)key_of(l[e]) << 32 | (uint32_t)~(uint32_t)(i + e));
@@ -440,7 +450,7 @@ __device__ __forceinline__ Found reach(Shared &s, const Row<T> &row, const Scale
         int its;
         // (the step's places lie between 4 * step - 2 and 4 * step + 6 below 0; an infinite logit's is none)
         if (scale.weight(l, s.table, own, its) && its == step)
-            part = min(max((int)(((scale.most == INFINITY ? 0.0 : -scale.place(l)) - (4 * step - 2)) * 32.0), 0), 255);
+            part = min(max((int)((-scale.place(l) - (4 * step - 2)) * 32.0), 0), 255);
     }
     const bool many = candidates > 64;   // a 256th of the step first: each of its members is held against the others
     if (many && tid < 256) {
@@ -533,13 +543,15 @@ __device__ __forceinline__ Scale scale_of(const Args &a, const Asked &ask, const
 {
     Scale s;
     s.most = v.most;
+    s.origin = fmin((double)v.most, 0x1p128);
     s.inverse = ask.greedy ? 1e30 : ask.t == INFINITY ? 1e-300 : 1.0 / (double)ask.t;
-    s.fractions = s.inverse * (kFractions * 1.4426950408889634);
+    s.fractions = v.most == INFINITY ? 1e300 : s.inverse * (kFractions * 1.4426950408889634);
     s.bits = a.bits;
+    s.least = -(double)(kFractions * (a.bits + 2));
     const float mean = v.total / v.number, spread = sqrtf(fmaxf(v.square / v.number - mean * mean, 0.0f));
     const float reach = fmaxf((v.most - mean) * a.near_share, v.most - mean - a.near_spread * spread);
     const float near_ = reach * (float)fmin(s.fractions * 0.25, 1e30);
-    s.near_steps = near_ < (float)kSteps ? (int)near_ + 1 : kSteps;
+    s.near_steps = min(near_ < (float)kSteps ? (int)near_ + 1 : kSteps, 64 * (a.bits + 1) + 1);   // (none without a weight)
     return s;
 }
 
@@ -586,7 +598,7 @@ __device__ Survey survey(Shared &s, const Row<T> &row)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float most = -INFINITY, total = 0.0f, square = 0.0f, number = 0.0f;
-    row.raw_pieces([&](int piece, const u32x4 &raw, bool inside) {
+    row.template raw_pieces<false>([&](int piece, const u32x4 &raw, bool inside) {
         if (inside) {
             const float first = logit_of(*(const T *)&raw);
             most = fmaxf(most, largest_of<T>(raw));
@@ -639,25 +651,29 @@ __device__ void clear(Shared &s)
 template <typename T>
 __device__ void histogram(Shared &s, const Row<T> &row, const Scale &scale, const Asked &ask)
 {
-    row.by_pieces([&](const float (&l)[Row<T>::kPiece], int i) {
-        u64 w[Row<T>::kPiece];
-        int step[Row<T>::kPiece];
-        bool live[Row<T>::kPiece];
+    row.template by_pieces<true>([&](const float (&l)[Row<T>::kPiece], int i) {
+        constexpr int P = Row<T>::kPiece;
+        u64 w[P];
+        int step[P];
 #pragma unroll
-        for (int e = 0; e < Row<T>::kPiece; ++e) {
-            live[e] = scale.weight(l[e], s.table, w[e], step[e]);
-            asm volatile("" : "+v"(w[e]));   // (formed side by side, not each behind a branch of its own)
+        for (int e = 0; e < P; ++e) {
+            scale.weight(l[e], s.table, w[e], step[e]);
+            asm volatile("" : "+v"(w[e]));   // (all formed before the first is put to use)
         }
 #pragma unroll
-        for (int e = 0; e < Row<T>::kPiece; ++e) {
-            if (!live[e]) continue;
-            atomicAdd(&s.sum[step[e]], w[e]);
-            if (ask.k >= kCounted) atomicAdd(&s.count[step[e]], 1u);
+        for (int e = 0; e < P; ++e)
+            if (w[e]) atomicAdd(&s.sum[step[e]], w[e]);
+        if (ask.k >= kCounted) {
+#pragma unroll
+            for (int e = 0; e < P; ++e)
+                if (w[e]) atomicAdd(&s.count[step[e]], 1u);
+        }
+#pragma unroll
+        for (int e = 0; e < P; ++e)
             if (step[e] < scale.near_steps) {
                 const uint32_t at = atomicAdd(&s.near_count, 1u);
                 if (at < (uint32_t)kNear) s.near_[at] = (u64)key_of(l[e]) << 32 | (uint32_t)~(uint32_t)(i + e);
             }
-        }
     });
 }
 
