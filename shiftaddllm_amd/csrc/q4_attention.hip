@@ -134,12 +134,19 @@ __device__ __forceinline__ uint32_t word_of(uint32_t codes)
     return w;
 }
 
+// Four codes of 4 bits each as bytes.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t codes)
+{
+    const uint32_t pairs = (codes & 0xffu) | (codes & 0xff00u) << 8;
+    return (pairs & 0x000f000fu) | (pairs & 0x00f000f0u) << 4;
+}
+
 // Rows of the held values of tokens first .. past - 1 that are passed over: zeros.
-template <int HD>
+template <int HD, int THREADS>
 __device__ __forceinline__ void clear_held(const Args &a, int b, int kvh, int n, int first, int past)
 {
     if (!a.k_held && !a.v_held) return;
-    for (int u = threadIdx.x; u < (past - first) * (HD / 8); u += kThreads) {
+    for (int u = threadIdx.x; u < (past - first) * (HD / 8); u += THREADS) {
         const int token = first + u / (HD / 8);
         if (token < n) continue;
         const size_t at = (((size_t)b * a.tokens + token) * a.kv_heads + kvh) * HD + u % (HD / 8) * 8;
@@ -148,13 +155,13 @@ __device__ __forceinline__ void clear_held(const Args &a, int b, int kvh, int n,
     }
 }
 
-// The new tokens of a (sequence, kv head) pair whose positions lie in a block of the cache, by a workgroup of kThreads that alone writes the
+// The new tokens of a (sequence, kv head) pair whose positions lie in a block of the cache, by a workgroup of THREADS that alone writes the
 // block, so that words that hold other positions too can be read, changed and written.  Lanes 4 i .. 4 i + 3 take a group of 32 numbers; the
 // values' codes meet by positions in LDS (`code`: kBlock rows of HD + 4 bytes).
-template <int G>
+template <int G, int THREADS>
 __device__ void append_block(const Args &a, int b, int kvh, int pair, int start, int n, int block, uint8_t *code)
 {
-    constexpr int HD = 32 * G, kStride = HD + 4, kWords = (128 * G + kThreads - 1) / kThreads;
+    constexpr int HD = 32 * G, kStride = HD + 4, kWords = (128 * G + THREADS - 1) / THREADS;
     const int tid = threadIdx.x;
     const int first = block * kBlock - start;   // token of the block's first position
     const int from = max(0, -first), past = min(kBlock, n - first);
@@ -166,9 +173,9 @@ __device__ void append_block(const Args &a, int b, int kvh, int pair, int start,
     const bool whole = past - from == kBlock;
     uint32_t before[kWords];   // (asked for ahead)
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) before[i] = !whole && tid + i * kThreads < 128 * G ? v_codes[tid + i * kThreads] : 0;
+    for (int i = 0; i < kWords; ++i) before[i] = !whole && tid + i * THREADS < 128 * G ? v_codes[tid + i * THREADS] : 0;
 
-    for (int u = tid; u < (past - from) * G * 4; u += kThreads) {
+    for (int u = tid; u < (past - from) * G * 4; u += THREADS) {
         const int quad = u % 4, t = u / 4 % G, p = from + u / (4 * G), token = first + p, d = 32 * t + 8 * quad;
         const _Float16 *kh = a.k + b * a.k_stride[0] + token * a.k_stride[1] + (size_t)kvh * HD;
         const _Float16 *vh = a.v + b * a.v_stride[0] + token * a.v_stride[1] + (size_t)kvh * HD;
@@ -176,8 +183,8 @@ __device__ void append_block(const Args &a, int b, int kvh, int pair, int start,
         const f16x8 v = *(const f16x8 *)(vh + d);
         const Held hk = quantise(rotated(kh, a.cos_t + angle, a.sin_t + angle, d, HD)), hv = quantise(v);
         k_codes[(p * 4 + quad) * G + t] = word_of(hk.codes);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) code[p * kStride + d + i] = (uint8_t)((hv.codes >> (4 * i)) & 15u);
+        *(uint32_t *)(code + p * kStride + d) = bytes_of(hv.codes);
+        *(uint32_t *)(code + p * kStride + d + 4) = bytes_of(hv.codes >> 16);
         if (quad == 0) {
             const f16x2 pair_of = {hk.scale, hk.low};
             k_scales[p * G + t] = __builtin_bit_cast(uint32_t, pair_of);
@@ -192,7 +199,7 @@ __device__ void append_block(const Args &a, int b, int kvh, int pair, int start,
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
-        const int u = tid + i * kThreads;
+        const int u = tid + i * THREADS;
         if (u >= 128 * G) break;
         const int t = u % (2 * G), column = u / (2 * G) % 16, quad = u / (32 * G);
         uint32_t fresh = 0, mask = 0;
@@ -209,16 +216,19 @@ __device__ void append_block(const Args &a, int b, int kvh, int pair, int start,
 
 // The new tokens of prompts: one workgroup per block of the cache that they fall into.
 template <int G>
-__global__ void __launch_bounds__(kThreads) append_kernel(const Args a)
+constexpr int kAppendThreads = G >= 4 ? 512 : 256;
+
+template <int G>
+__global__ void __launch_bounds__(kAppendThreads<G>) append_kernel(const Args a)
 {
-    __shared__ uint8_t code[kBlock * (32 * G + 4)];
+    __shared__ __attribute__((aligned(4))) uint8_t code[kBlock * (32 * G + 4)];
     const int pair = blockIdx.x % a.pairs, part = blockIdx.x / a.pairs;
     const int b = pair / a.kv_heads, kvh = pair % a.kv_heads;
     int start;
     const int n = live_tokens(a, b, start);
-    clear_held<32 * G>(a, b, kvh, n, min(part * kBlock, a.tokens), min((part + 1) * kBlock, a.tokens));
+    clear_held<32 * G, kAppendThreads<G>>(a, b, kvh, n, min(part * kBlock, a.tokens), min((part + 1) * kBlock, a.tokens));
     const int block = start / kBlock + part;
-    if (n > 0 && block * kBlock < start + n) append_block<G>(a, b, kvh, pair, start, n, block, code);
+    if (n > 0 && block * kBlock < start + n) append_block<G, kAppendThreads<G>>(a, b, kvh, pair, start, n, block, code);
 }
 
 // Two held values from bits 4 I .. of either half of a word (I = 0, 1): the code, put into the low bits of the significand of 1024 (64), is
@@ -374,13 +384,13 @@ __global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attenti
     const int blocks = (limit_high + kBlock) / kBlock;
     const int per = blocks_per_split(a, blocks, kWaves);
     const int begin = split * per, end = min(begin + per, blocks);
-    if (a.fused && split == 0) clear_held<HD>(a, b, kvh, n, 0, a.tokens);
+    if (a.fused && split == 0) clear_held<HD, kThreads>(a, b, kvh, n, 0, a.tokens);
     if (a.splits > 1 && begin >= end) return;                                  // (nobody reads its part)
 
     // Fused: the one tile of a pair's rows; the workgroup whose blocks new tokens fall into appends them before anything is read.
     if (a.fused && n > 0 && start / kBlock < end) {
         for (int fresh = max(start / kBlock, begin); fresh < end; ++fresh) {
-            append_block<G>(a, b, kvh, pair, start, n, fresh, (uint8_t *)joined);
+            append_block<G, kThreads>(a, b, kvh, pair, start, n, fresh, (uint8_t *)joined);
             __syncthreads();
         }
     }
@@ -864,7 +874,7 @@ int lutgemm_q4_attention_f16(const lutgemm_q4_attention *c, void *workspace, siz
         int status = LUTGEMM_OK;
         if (!plan.fused) {
             const long parts = (a.tokens + kBlock - 1) / kBlock + 1;
-            hipLaunchKernelGGL(append_kernel<G>, dim3((unsigned)(parts * a.pairs)), dim3(kThreads), 0, hs, a);
+            hipLaunchKernelGGL(append_kernel<G>, dim3((unsigned)(parts * a.pairs)), dim3(kAppendThreads<G>), 0, hs, a);
             status = launch_status();
             if (status != LUTGEMM_OK) return status;
         }
