@@ -699,7 +699,8 @@ int lutgemm_decode_silu_mul_f16(const void *gate, const void *up, void *out, siz
  * softmax(q k^T / sqrt(head_dim)) v, sums in fp32.  Tokens beyond a sequence's count, tokens at positions outside the cache,
  * and all of a sequence whose start is negative (an idle slot) are passed over: nothing is appended, and their rows of out,
  * k_held and v_held are zeros.  Positions that are not attended to have no influence, whatever the cache holds there; a
- * sequence's earlier positions are the caller's to have filled.  out, k_held, v_held and the cache may not overlap anything.
+ * sequence's earlier positions are the caller's to have filled.  out, k_held, v_held and the cache may not overlap anything
+ * (LUTGEMM_EINVAL).
  *
  * `workspace`: lutgemm_q4_attention_workspace bytes (0: none needed; the size does not depend on what start and counts
  * hold), 16-byte aligned, of any contents, in use until the call's work is done.  Nothing is allocated, the launches

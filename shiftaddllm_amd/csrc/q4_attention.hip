@@ -792,6 +792,31 @@ int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int 
     return LUTGEMM_OK;
 }
 
+struct Span {
+    uintptr_t from, past;
+};
+
+bool overlap(const Span &a, const Span &b) { return a.from < b.past && b.from < a.past; }
+
+// Whether what a call writes lies apart from all else that it is given.
+bool written_apart(const lutgemm_q4_attention *c)
+{
+    auto span = [](const void *p, size_t bytes) { return Span{(uintptr_t)p, (uintptr_t)p + (p ? bytes : 0)}; };
+    auto rows = [&](const void *p, const int64_t (&stride)[2], int heads) {
+        return span(p, 2 * ((size_t)(c->batch - 1) * stride[0] + (size_t)(c->tokens - 1) * stride[1] + (size_t)heads * c->head_dim));
+    };
+    const size_t tokens = (size_t)c->batch * c->tokens, table = (size_t)c->max_positions * c->head_dim * 2;
+    const size_t held = tokens * c->kv_heads * c->head_dim * 2;
+    const Span all[] = {span(c->cache, lutgemm_q4_cache_bytes(c->batch, c->kv_heads, c->max_positions, c->head_dim)),
+                        span(c->out, tokens * c->heads * c->head_dim * 2), span(c->k_held, held), span(c->v_held, held),
+                        rows(c->q, c->q_stride, c->heads), rows(c->k, c->k_stride, c->kv_heads), rows(c->v, c->v_stride, c->kv_heads),
+                        span(c->cos_table, table), span(c->sin_table, table), span(c->start, (size_t)c->batch * 8), span(c->counts, (size_t)c->batch * 4)};
+    for (int i = 0; i < 4; ++i)
+        for (int j = i + 1; j < (int)(sizeof(all) / sizeof(all[0])); ++j)
+            if (overlap(all[i], all[j])) return false;
+    return true;
+}
+
 bool strides_fit(const int64_t (&s)[2], const void *p)
 {
     return aligned16(p) && s[0] % 8 == 0 && s[1] % 8 == 0;
@@ -837,6 +862,7 @@ int lutgemm_q4_attention_f16(const lutgemm_q4_attention *c, void *workspace, siz
         !aligned16(c->v_held) || ((uintptr_t)c->start & 7u) || ((uintptr_t)c->counts & 3u) || (sizes.workspace > 0 && !aligned16(workspace)) ||
         !strides_fit(c->q_stride, c->q) || !strides_fit(c->k_stride, c->k) || !strides_fit(c->v_stride, c->v))
         return LUTGEMM_EALIGN;
+    if (!written_apart(c)) return LUTGEMM_EINVAL;
     Args a{};
     a.cache = (uint8_t *)c->cache;
     a.q = (const _Float16 *)c->q;

@@ -366,7 +366,8 @@ class LutDecoder(nn.Module):
             check(lib.lutgemm_decode_rmsnorm_f16(x.data_ptr(), w.data_ptr(), h.data_ptr(), x.shape[0], cfg.hidden, cfg.rms_eps, None, 0, sp))
             return h
 
-        x = self.embed[input_ids.to(dev).reshape(-1)]
+        there = torch.arange(T, device=dev) < count.unsqueeze(1)      # (whatever stands behind a sequence's tokens is no index)
+        x = self.embed[torch.where(there, input_ids.to(dev), 0).reshape(-1)]
         for li, blk in enumerate(self.blocks):
             h = norm(x, blk.input_norm)
             q, k, v = (l(h, ids).view(B, T, -1) for l in (blk.q_proj, blk.k_proj, blk.v_proj))
@@ -597,7 +598,7 @@ class LutDecoder(nn.Module):
         """One token per sequence at `position`; with a cache of 4 bits also a position for every sequence (a list or a tensor in
         host memory), negative for one that is idle."""
         P = self.cfg.max_positions
-        if isinstance(position, int):
+        if not isinstance(position, (list, tuple)) and not (isinstance(position, torch.Tensor) and position.dim() > 0):
             # the attention kernel clamps the position into the cache: past its end it would
             # overwrite the last slot and return plausible but wrong logits
             if not 0 <= position < P:

@@ -173,7 +173,7 @@ class LutLinear(nn.Module):
         return buf
 
     def forward(self, x, adapter_ids=None):
-        """W_q x + bias; with `adapter_ids` (int32, one per row of x) plus, row by row, the product of the adapter of `self.adapters` that
+        """W_q x + bias; with `adapter_ids` (int32 or int64, one per row of x) plus, row by row, the product of the adapter of `self.adapters` that
         the id names (none where it is not one of them).  Then x is rounded to fp16 first, and the sum is formed in fp16 rows:
         the layer's result and the adapter's are each rounded once."""
         if adapter_ids is not None:
@@ -202,7 +202,9 @@ class LutLinear(nn.Module):
             raise ValueError(f"adapters of a {bank.K} -> {bank.N} projection beside a {self.K} -> {self.N} layer")
         half = x if x.dtype is torch.float16 else x.to(torch.float16)
         y = LutLinear.forward(self, half)
-        y = bank(half, adapter_ids.reshape(-1).to(torch.int32), y, y)
+        if adapter_ids.dtype is torch.int64:
+            adapter_ids = adapter_ids.clamp(-1, bank.count).to(torch.int32)   # (an id beyond 32 bits is no adapter's either)
+        y = bank(half, adapter_ids.reshape(-1), y, y)
         return y if x.dtype is torch.float16 else y.to(x.dtype)
 
     def extra_repr(self):

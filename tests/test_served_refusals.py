@@ -238,3 +238,16 @@ def test_linear_layers_keep_their_state():
         lin(torch.zeros((1, 64)), torch.zeros(1, dtype=torch.int32))
     lin.adapters = AdapterBank(64, 32, 8, 2)
     assert sorted(lin.state_dict()) == ["adapters.down", "adapters.scale", "adapters.up", "alpha", "binaryWeight"]
+
+
+def test_attention_refuses_outputs_that_overlap(lib):
+    """What a call writes may not lie in anything else that it is given, nor in what it writes besides."""
+    place = {n: BASE + i * (1 << 20) for i, n in enumerate(("cache", "q", "k", "v", "cos_table", "sin_table", "start", "counts", "out", "k_held", "v_held"))}
+    call = lambda **kw: lib.lutgemm_q4_attention_f16(ctypes.byref(attention(**{**place, **kw})), None, 0, None)
+    size = dict(cache=2 * 2 * 2 * 40 * 128, out=2 * 512 * 2, k_held=2 * 256 * 2, v_held=2 * 256 * 2)
+    for name, bytes_ in size.items():
+        for other in place:
+            if other == name:
+                continue
+            assert call(**{name: place[other]}) == E_INVAL, (name, other)
+            assert call(**{other: place[name] + bytes_ - 16}) == E_INVAL, (name, other)
