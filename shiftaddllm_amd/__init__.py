@@ -5,6 +5,10 @@ Layout of the package:
   csrc/lutgemm_torch.cpp     Python module `lutgemm` with the reference signatures
   lut_gemm/quant.py          LutLinear, make_lut, load_lut
   lut_gemm/kernel.py         pack / unpack / convert / checkpoint loaders
+  lut_gemm/adapters.py       AdapterBank: low-rank adapters of many requests beside a LutLinear
+  kv_cache.py                Q4Cache: keys and values held in 4 bits, appending and attention
+  sampling.py                sample: temperature, top-k, top-p and min-p from given random numbers
+  decode.py                  LutDecoder, the decode harness in which all of these run
   workload.py                seeded synthetic BCQ problems for tests and benchmarks
   build.py                   in-tree build of the two shared objects
 
