@@ -117,9 +117,11 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Args args)
         const int id = m < p.M ? adapter_of(p, m) : 0;
         return id < 0 ? p.adapters : id;
     };
+    // (a row's kind and place stay in registers where a thread has no more rows than it looks at at a time)
+    const bool once = p.M <= kRows * 1024;
+    int kind[kRows], places[kRows];
     __syncthreads();
     for (int m0 = tid; m0 - tid < p.M; m0 += kRows * 1024) {
-        int kind[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) kind[i] = kind_of(m0 + 1024 * i);
 #pragma unroll
@@ -131,9 +133,11 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Args args)
             int place = 0;
             if (lane == 0 && same) place = atomicAdd(&rows[its], __popcll(same));
             place = __builtin_amdgcn_readfirstlane(place) + __popcll(same & ((1ull << lane) - 1));
+            places[i] = 0;
             if (m >= p.M) continue;
             if (kind[i] != its) place = atomicAdd(&rows[kind[i]], 1);
-            p.places[m] = place;
+            places[i] = place;
+            if (!once) p.places[m] = place;
         }
     }
     __syncthreads();
@@ -185,15 +189,16 @@ __global__ void __launch_bounds__(1024) sort_kernel(const Args args)
     for (int t = tiles + tid; t < p.slots; t += 1024) p.tiles[t] = {-1, 0, 0};
     __syncthreads();
     for (int m0 = tid; m0 < p.M; m0 += kRows * 1024) {
-        int kind[kRows], place[kRows];
+        if (!once) {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            kind[i] = kind_of(m0 + 1024 * i);
-            place[i] = p.places[min(m0 + 1024 * i, p.M - 1)];
+            for (int i = 0; i < kRows; ++i) {
+                kind[i] = kind_of(m0 + 1024 * i);
+                places[i] = p.places[min(m0 + 1024 * i, p.M - 1)];
+            }
         }
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-            if (m0 + 1024 * i < p.M) p.order[rows[kind[i]] + place[i]] = m0 + 1024 * i;
+            if (m0 + 1024 * i < p.M) p.order[rows[kind[i]] + places[i]] = m0 + 1024 * i;
     }
 }
 
