@@ -846,16 +846,27 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const Args a)
     const RowWork &work = a.work[r];
     const Row<T> row((const T *)a.logits + r * a.row_stride, a.vocab, 0, 1);
     const Asked ask(a, r);
+    // (all that may be wanted is asked for at once, before anything is known of the row: entries of the list that are not there have no meaning)
+    constexpr int kSome = 2;
+    u64 sums[kPerThread], some[kSome];
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) sums[i] = work.sum[tid + i * kThreads];
+#pragma unroll
+    for (int i = 0; i < kSome; ++i) some[i] = work.near_[tid + i * kThreads];
+    const uint32_t listed = work.near_count;
+    const double power = tid < kFractions ? kTable.power[tid] : 0.0;
     Scale scale;
     if (!scale_of_row(a, ask, work, scale)) return nothing(a, r);
-    for (int b = tid; b < kSteps; b += kThreads) {
-        s.sum[b] = work.sum[b];
-        s.count[b] = work.count[b];
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+        s.sum[tid + i * kThreads] = sums[i];
+        s.count[tid + i * kThreads] = ask.k >= kCounted ? work.count[tid + i * kThreads] : 0;
     }
-    const uint32_t listed = work.near_count;
+#pragma unroll
+    for (int i = 0; i < kSome; ++i) s.near_[tid + i * kThreads] = some[i];
     if (listed <= (uint32_t)kNear)
-        for (uint32_t i = tid; i < listed; i += kThreads) s.near_[i] = work.near_[i];
-    if (tid < kFractions) s.table[tid] = kTable.power[tid];
+        for (uint32_t i = tid + kSome * kThreads; i < listed; i += kThreads) s.near_[i] = work.near_[i];
+    if (tid < kFractions) s.table[tid] = power;
     if (tid == 0) {
         s.near_count = listed;
         s.least_sum = 0;
