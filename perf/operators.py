@@ -183,8 +183,9 @@ def prepare(case, seed):
     elif case["op"] == "sample":
         R, V = case["rows"], case["vocab"]
         logits = normal(R, V) * 2.2 - 3
-        at = torch.randint(0, V, (R, 40), generator=g, device=DEVICE)
-        logits.scatter_(1, at, normal(R, 40) * 2.5 + 7)                              # what the context speaks for
+        # what the context speaks for: one token from every fortieth of the vocabulary (a token twice would get either of two values)
+        at = torch.randint(0, V // 40, (R, 40), generator=g, device=DEVICE) + torch.arange(40, device=DEVICE) * (V // 40)
+        logits.scatter_(1, at, normal(R, 40) * 2.5 + 7)
         logits.masked_fill_(uniform(R, V) < 0.01, float("-inf"))                     # banned tokens
         s["logits"] = logits.to(_DTYPES[case["dtype"]])
         s["uniform"] = uniform(R)
