@@ -167,7 +167,7 @@ class LutDecoder(nn.Module):
             self.register_buffer("v_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
         else:
             self.q4 = [Q4Cache(batch, cfg.kv_heads, cfg.max_positions, hd, dev) for _ in range(cfg.layers)]
-            self.register_buffer("starts", torch.zeros((batch,), dtype=torch.long, device=dev), persistent=False)
+            self.register_buffer("starts", torch.full((batch,), -1, dtype=torch.long, device=dev), persistent=False)
         if adapters is not None:
             self.register_buffer("adapter_ids", torch.full((batch,), -1, dtype=torch.int32, device=dev), persistent=False)
         if sampling is not None:
@@ -243,8 +243,8 @@ class LutDecoder(nn.Module):
     # ---- one token ---------------------------------------------------------------------------
     @torch.no_grad()
     def step(self):
-        """Consumes self.ids [B] at position self.pos [1] (self.starts [B] with a cache of 4 bits); writes self.logits [B, V]
-        and, with sampling, self.next_ids and self.next_logprob [B]."""
+        """Consumes self.ids [B] at position self.pos [1] (self.starts [B] with a cache of 4 bits: negative, as at first, for idle
+        sequences); writes self.logits [B, V] and, with sampling, self.next_ids and self.next_logprob [B]."""
         if self.glue == "torch":
             self._step_torch()
         elif self.has_adapters:
@@ -579,14 +579,23 @@ class LutDecoder(nn.Module):
     @torch.no_grad()
     def capture(self):
         """Capture step() in a HIP graph (after one eager run on the capture stream,
-        which also sizes the LUT-GEMM workspace of that stream)."""
+        which also sizes the LUT-GEMM workspace of that stream).  With a cache of 4 bits the eager run leaves the caches, the
+        logits and the sequences' positions as they are, with sampling also what was drawn last: prompts may have been taken already."""
         self._stream = torch.cuda.Stream()
         # weights, caches and the step's input buffers were filled on the creating stream:
         # without this wait the first step may read them (the token ids among them, which
         # index the embedding table) before they have been written
         self._stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(self._stream):
+            kept = [self.starts, self.logits] if self.kv_bits == 4 else []
+            if self.sampling is not None:
+                kept += [self.next_ids, self.next_logprob]
+            before = [t.clone() for t in kept]
+            if self.kv_bits == 4:
+                self.starts.fill_(-1)                          # (all idle: nothing is appended; the launches depend on sizes alone)
             self.step()
+            for t, b in zip(kept, before):
+                t.copy_(b)
         self._stream.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=self._stream):
