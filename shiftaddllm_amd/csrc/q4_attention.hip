@@ -281,12 +281,15 @@ __device__ __forceinline__ void load_queries(const Args &a, int b, int kvh, int 
 // Of one row a lane: the reference (a score), the sum of weights 2^(factor * (score - reference)), and the weighted values.
 template <int G>
 struct RowState {
-    float reference, sum;
+    float reference, sum, off;   // off: -reference * factor, or 0 where scores are brought to the reference ahead (`far`)
+    bool far;                    // of the wave: factor * reference is so large in a row that its rounding in `off` would count
     f32x4 acc[2 * G];
-    __device__ __forceinline__ void clear()
+    __device__ __forceinline__ void clear(float factor)
     {
         reference = -1e30f;
         sum = 0.0f;
+        off = -reference * factor;
+        far = false;
 #pragma unroll
         for (int t = 0; t < 2 * G; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -306,14 +309,23 @@ struct RowState {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float raised = fmaxf(reference, most), keep = __builtin_amdgcn_exp2f((reference - raised) * factor);
             reference = raised;
+            // A weight is one fused sum, factor * score + off, where off is rounded: by 2^-5 at most up to 2^20.  Beyond that it could make the row's
+            // largest weight any power of two: differences are formed first there, which are exact near the reference.  (Rows without a score
+            // yet, beyond 2^60, do not count, nor do infinite ones: those are spoilt anyway.)
+            const float size = fabsf(reference * factor);
+            far = __any(size > 0x1p20f && size < 0x1p60f);
+            off = far ? 0.0f : -reference * factor;
             sum *= keep;
 #pragma unroll
             for (int t = 0; t < 2 * G; ++t) acc[t] *= keep;
         }
+        if (far) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) score[e / 4][e % 4] -= reference;
+        }
     }
     __device__ __forceinline__ f16x8 weights(const f32x4 (&score)[2], float factor)
     {
-        const float off = -reference * factor;
         f16x8 w;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -401,10 +413,10 @@ __global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attenti
     f16x8 q[RT][G];
     int limit[RT];
     load_queries<G, RT>(a, b, kvh, start, row0, live_rows, q, limit);
+    const float factor = 1.4426950408889634f / sqrtf((float)HD);
     RowState<G> state[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) state[rt].clear();
-    const float factor = 1.4426950408889634f / sqrtf((float)HD);
+    for (int rt = 0; rt < RT; ++rt) state[rt].clear(factor);
     const uint8_t *cache = a.cache + (size_t)pair * a.blocks * (size_t)(1280 * G);
 
     uint32_t k_codes[2][G], k_scales[2][G], v_codes[2 * G], v_scales[2 * G][4];
@@ -608,10 +620,10 @@ __global__ void __launch_bounds__(64 * W, 2) prompt_kernel(const Args a)
     f16x8 q[RT][G];
     int limit[RT];
     load_queries<G, RT>(a, b, kvh, start, row0, live_rows, q, limit);
+    const float factor = 1.4426950408889634f / sqrtf((float)HD);
     RowState<G> state[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) state[rt].clear();
-    const float factor = 1.4426950408889634f / sqrtf((float)HD);
+    for (int rt = 0; rt < RT; ++rt) state[rt].clear(factor);
     f32x4 score[RT][2];
     f16x8 operand[2 * G];
     auto multiply_keys = [&](f32x4 (&to)[RT][2]) {
