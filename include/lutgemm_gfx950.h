@@ -696,7 +696,9 @@ int lutgemm_decode_silu_mul_f16(const void *gate, const void *up, void *out, siz
  *                cache now holds for the new tokens
  * Token i of a sequence stands at position start + i.  Its key is rotated (rounded to fp16) and appended with its value, and
  * its query, rotated likewise, attends to the held values of positions 0 .. start + i, its own among them:
- * softmax(q k^T / sqrt(head_dim)) v, sums in fp32.  Tokens beyond a sequence's count, tokens at positions outside the cache,
+ * softmax(q k^T / sqrt(head_dim)) v, sums in fp32; the softmax's weights are rounded to fp16 for their product with v: by half a
+ * step, 2^-11 of each, at most, and where they are below 2^-21 of the row's largest by 2^-32 of that.
+ * Tokens beyond a sequence's count, tokens at positions outside the cache,
  * and all of a sequence whose start is negative (an idle slot) are passed over: nothing is appended, and their rows of out,
  * k_held and v_held are zeros.  Positions that are not attended to have no influence, whatever the cache holds there; a
  * sequence's earlier positions are the caller's to have filled.  out, k_held, v_held and the cache may not overlap anything

@@ -9,8 +9,11 @@
 // A held value is one fp16 number, fp16(minimum + scale * code); it is formed in registers (a shift, and-or, an exact
 // subtraction and an fma for two values) and multiplied exactly, sums in fp32.
 // Softmax keeps a reference per row, not the exact maximum: it is raised only when a score exceeds it by 2^8, so that most
-// blocks need no exchange between lanes.  Weights, at most 2^8, are rounded to fp16 for the matrix product (half a step, 2^-11 relative,
-// where they are 2^-14 or more; the error of a sum over many positions averages out); their sum is formed in fp32 from the unrounded ones.
+// blocks need no exchange between lanes.  Weights are held 2^7 times as large (which cancels in every quotient), so that they take up fp16's range
+// where they are rounded for the matrix product: 2^15 at most, half a step (2^-11 relative) down to 2^-21 of the reference's weight, 2^-32 of
+// that below: 2^20 such positions come to 2^-12 of the largest weight.  (With the reference's weight at one, the tail of a row with a
+// dominant position was lost: 8192 positions at 2^-26 each came out as nothing.)  The error of a sum over many positions averages out.  Their sum is
+// formed in fp32 from the unrounded ones.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -34,6 +37,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBlock = 32;              // positions of a block of the cache
 constexpr float kLargest = 60000.0f;    // of a held number
 constexpr float kSlack = 8.0f;          // by which (in powers of two) a score may exceed its row's reference
+constexpr float kLift = 7.0f;           // by which weights are held larger
 
 struct Args {
     uint8_t *cache;
@@ -278,17 +282,17 @@ __device__ __forceinline__ void load_queries(const Args &a, int b, int kvh, int 
     }
 }
 
-// Of one row a lane: the reference (a score), the sum of weights 2^(factor * (score - reference)), and the weighted values.
+// Of one row a lane: the reference (a score), the sum of weights 2^(factor * (score - reference) + kLift), and the weighted values.
 template <int G>
 struct RowState {
-    float reference, sum, off;   // off: -reference * factor, or 0 where scores are brought to the reference ahead (`far`)
+    float reference, sum, off;   // off: kLift - reference * factor, or kLift where scores are brought to the reference ahead (`far`)
     bool far;                    // of the wave: factor * reference is so large in a row that its rounding in `off` would count
     f32x4 acc[2 * G];
     __device__ __forceinline__ void clear(float factor)
     {
         reference = -1e30f;
         sum = 0.0f;
-        off = -reference * factor;
+        off = kLift - reference * factor;
         far = false;
 #pragma unroll
         for (int t = 0; t < 2 * G; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -309,12 +313,12 @@ struct RowState {
             most = fmaxf(most, __shfl_xor(most, 32));
             const float raised = fmaxf(reference, most), keep = __builtin_amdgcn_exp2f((reference - raised) * factor);
             reference = raised;
-            // A weight is one fused sum, factor * score + off, where off is rounded: by 2^-5 at most up to 2^20.  Beyond that it could make the row's
-            // largest weight any power of two: differences are formed first there, which are exact near the reference.  (Rows without a score
-            // yet, beyond 2^60, do not count, nor do infinite ones: those are spoilt anyway.)
+            // A weight is one fused sum, factor * score + off, where off is rounded: by 2^-4 at most up to 2^20, so that weights stay below 2^15.1.
+            // Beyond that it could make the row's largest weight any power of two: differences are formed first there, which are exact near the
+            // reference.  (Rows without a score yet, beyond 2^60, do not count, nor do infinite ones: those are spoilt anyway.)
             const float size = fabsf(reference * factor);
             far = __any(size > 0x1p20f && size < 0x1p60f);
-            off = far ? 0.0f : -reference * factor;
+            off = far ? kLift : kLift - reference * factor;
             sum *= keep;
 #pragma unroll
             for (int t = 0; t < 2 * G; ++t) acc[t] *= keep;
