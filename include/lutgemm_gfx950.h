@@ -750,8 +750,9 @@ int lutgemm_describe_q4_attention_plan(int batch, int tokens, int heads, int kv_
  * temperature <= 0: the first token of the order, logprob 0.  A row without weight (all -inf or NaN): id -1, logprob -inf.
  * A parameter that is NaN counts as off (temperature as 0, uniform as 0).  uniform is taken into [0, 1); what rounding leaves
  * behind the last sum is the last token left.
- * Weights are formed in 64 bits, held to 2^-43 of the largest (2^-51 up to 4096 tokens) and added as whole numbers: the same result
- * whatever the order, and the one that the formulas give in 64 bits but for numbers that lie within about 2^-40 of a border.
+ * Weights are formed in 64 bits, held as whole numbers of 2^-b of the largest (b = 63 - ceil(log2 vocab), at most 51: 43 for 2^20 tokens)
+ * and added as such: the same result whatever the order, and the one that the formulas give in 64 bits but for numbers that lie near a
+ * border: within vocab * 2^-(b + 1) of the largest weight (2^-40 for 2^12 tokens, 2^-30 for 2^17) where all are rounded alike, mostly far nearer.
  *   logits     [rows][vocab] of logits_type (LUTGEMM_TYPE_*), row_stride elements between rows, aligned to their own size
  *   temperature, top_p, min_p, uniform  float [rows], top_k int32 [rows], device; all but uniform may be NULL (1, off)
  *   ids        int64 [rows]; logprob  NULL, or float [rows]
