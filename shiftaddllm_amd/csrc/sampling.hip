@@ -126,10 +126,11 @@ struct Scale {
         step = -n >> 2;   // (larger logits in earlier ones)
         return w != 0;
     }
-    // Whether a logit is of a step, but for its last hundredth on either side (a difference's place in fp32 is off by 2^-22 of itself).
+    // Whether a logit is of a step, but for its last hundredth on either side (a difference's place in fp32 is off by 2^-22 of itself; half
+    // differences, since those of finite logits can lie beyond fp32's range).
     __device__ __forceinline__ bool near_step(float l, int step) const
     {
-        const float p = (most - l) * (float)(fractions * 0.25);
+        const float p = (0.5f * most - 0.5f * l) * (float)(fractions * 0.5);
         return !(p < (float)step - 0.135f) && (!(p > (float)step + 0.885f) || fractions >= 1e30);
     }
     __device__ __forceinline__ double exponent(float l) const { return l == most ? 0.0 : ((double)l - (double)most) * inverse; }
