@@ -777,7 +777,8 @@ int lutgemm_sample_tokens(const lutgemm_sampling *call, void *workspace, size_t 
  * ---- low-rank adapters beside a shared linear layer (no counterpart in the reference) -------------------------------------------
  * Every row takes the adapter that its id names, or none: a = ids[m],
  *   out[m][n] = fp16(base[m][n] + scale[a] * sum_r up[a][n][r] * h[r]),   h[r] = sum_k down[a][r][k] * x[m][k]
- * with h and the sums in fp32; out[m] = base[m] where a is not in 0 .. adapters - 1.
+ * with h and the sums in fp32; out[m] = base[m] where a is not in 0 .. adapters - 1.  Infinities and NaN come out as these formulas say, but
+ * for infinite numbers of up, which may give NaN instead.
  *   x [M][K], base [M][N], out [M][N] fp16, rows x_stride, base_stride, out_stride elements apart (x_stride a multiple of 8, the others
  *   of 4); x 16-byte aligned, base and out 8-byte aligned; out may be base itself, with its stride
  *   ids int32 [M], device;  down fp16 [adapters][rank][K], up fp16 [adapters][N][rank], 16-byte aligned;  scale float

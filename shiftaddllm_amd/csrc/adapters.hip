@@ -345,18 +345,19 @@ __global__ void __launch_bounds__(kThreads) up_kernel(const Args args)
                 v[i] += r < p.rank && live ? h[(size_t)s * p.M * p.rank + r] : 0.0f;
             }
         }
+        // (infinite ones are left out: they stay infinite whatever they are scaled by)
 #pragma unroll
-        for (int i = 0; i < RT * 2; ++i) most = fmaxf(most, fabsf(v[i]));
+        for (int i = 0; i < RT * 2; ++i) most = fabsf(v[i]) < INFINITY ? fmaxf(most, fabsf(v[i])) : most;
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-        // (a power of two not below the largest, inside what can be inverted; infinite rows stay as they are)
-        const int exponent = most > 0.0f && most < INFINITY ? min(max(__builtin_amdgcn_frexp_expf(most), -100), 100) : 0;
+        // (a power of two not below the largest, inside what can be inverted)
+        const int exponent = most > 0.0f ? min(max(__builtin_amdgcn_frexp_expf(most), -100), 100) : 0;
 #pragma unroll
         for (int i = 0; i < RT * 2; ++i) {
             const float scaled = __builtin_amdgcn_ldexpf(v[i], -exponent);
             const _Float16 hi = (_Float16)scaled;
             high[row][part + 16 * i] = hi;
-            low[row][part + 16 * i] = (_Float16)(scaled - (float)hi);
+            low[row][part + 16 * i] = fabsf(scaled) < INFINITY ? (_Float16)(scaled - (float)hi) : (_Float16)0.0f;
         }
         if (part == 0) back[row] = __builtin_amdgcn_ldexpf(p.scale ? p.scale[id] : 1.0f, exponent);
     }
