@@ -41,7 +41,8 @@ struct RowWork {
     u64 sum[kSteps];
     u64 near_[kNear];
     uint32_t count[kSteps];
-    uint32_t near_count, unused[3];
+    uint32_t near_count;
+    int near_steps, unused[2];
     float most[kParts], total[kParts], square[kParts], number[kParts];   // of the parts
 };
 
@@ -557,7 +558,7 @@ __device__ __forceinline__ Scale scale_of(const Args &a, const Asked &ask, const
     const float mean = v.total / v.number, spread = sqrtf(fmaxf(v.square / v.number - mean * mean, 0.0f));
     const float reach = fmaxf((v.most - mean) * a.near_share, v.most - mean - a.near_spread * spread);
     const float near_ = reach * (float)fmin(s.fractions * 0.25, 1e30);
-    s.near_steps = min(near_ < (float)kSteps ? (int)near_ + 1 : kSteps, 64 * (a.bits + 1) + 1);   // (none without a weight)
+    s.near_steps = min(near_ < (float)kSteps ? (int)fmaxf(near_, 0.0f) + 1 : kSteps, 64 * (a.bits + 1) + 1);   // (none without a weight)
     return s;
 }
 
@@ -834,6 +835,7 @@ __global__ void __launch_bounds__(kThreads) histogram_kernel(const Args a)
     const uint32_t own = s.near_count;
     if (tid == 0) {
         s.members = own ? atomicAdd(&work.near_count, own) : 0;
+        if (part == 0) work.near_steps = scale.near_steps;   // (handed on, not formed again: the list holds these steps and no others)
     }
     __syncthreads();
     for (uint32_t i = tid; i < own && s.members + i < (uint32_t)kNear && i < (uint32_t)kNear; i += kThreads) work.near_[s.members + i] = s.near_[i];
@@ -855,9 +857,11 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const Args a)
 #pragma unroll
     for (int i = 0; i < kSome; ++i) some[i] = work.near_[tid + i * kThreads];
     const uint32_t listed = work.near_count;
+    const int listed_steps = work.near_steps;
     const double power = tid < kFractions ? kTable.power[tid] : 0.0;
     Scale scale;
     if (!scale_of_row(a, ask, work, scale)) return nothing(a, r);
+    scale.near_steps = listed_steps;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
         s.sum[tid + i * kThreads] = sums[i];
