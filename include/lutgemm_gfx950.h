@@ -687,7 +687,9 @@ int lutgemm_decode_silu_mul_f16(const void *gate, const void *up, void *out, siz
  *
  * One call takes `tokens` new tokens of every sequence: a single one, a few, or a prompt.
  *   q, k, v      fp16 [batch][tokens][heads (kv_heads) * head_dim], strides in elements: *_stride[0] between sequences, [1]
- *                between tokens, multiples of 8, 0 or more; 16-byte aligned.  heads a multiple of kv_heads, at most 4096
+ *                between tokens, multiples of 8, 0 or more; 16-byte aligned.  heads a multiple of kv_heads, at most 4096.
+ *                Sizes at which a launch would have 2^32 work items (2^24 kv heads of all sequences, or 2^32 / 512 blocks that a
+ *                prompt's tokens fall into) are refused
  *   cos, sin     fp16 [max_positions][head_dim], the two halves of a row equal (rotate-half convention); 16-byte aligned
  *   start        int64 [batch], device: the position of a sequence's first new token
  *   counts       NULL (all `tokens`), or int32 [batch], device: how many of its tokens are there

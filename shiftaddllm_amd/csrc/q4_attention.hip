@@ -220,8 +220,10 @@ __device__ void append_block(const Args &a, int b, int kvh, int pair, int start,
 
 // The new tokens of prompts: one workgroup per block of the cache that they fall into, a thread for eight numbers of a token's key and value
 // (two prompts of 2048 on 8 kv heads: 39 MB in 14 us; 256 threads, which take two turns, 15.5).
+constexpr int append_threads(int groups) { return groups >= 4 ? 512 : 256; }
+
 template <int G>
-constexpr int kAppendThreads = G >= 4 ? 512 : 256;
+constexpr int kAppendThreads = append_threads(G);
 
 template <int G>
 __global__ void __launch_bounds__(kAppendThreads<G>) append_kernel(const Args a)
@@ -806,12 +808,15 @@ int plan_call(int batch, int tokens, int heads, int kv_heads, int head_dim, int 
     p->splits = (int)splits;
     p->row_tiles = s->tiles;
     p->launches = 1 + !p->fused + (splits > 1);
-    if (alone * splits > 0x7fffffffl || pairs * ((tokens + kBlock - 1) / kBlock + 1) > 0x7fffffffl) return LUTGEMM_EINVAL;
+    // (a launch takes fewer than 2^32 work items: refused here, before the first of a call's launches)
+    const long most_items = 0xffffffffl, append_parts = (tokens + kBlock - 1) / kBlock + 1;
+    if (alone * splits * p->threads > most_items || (!p->fused && pairs * append_parts * append_threads(head_dim / 32) > most_items) ||
+        (splits > 1 && pairs * rows * kThreads > most_items))
+        return LUTGEMM_EINVAL;
     p->workgroups = (int)(alone * splits);
     const size_t part_rows = (size_t)splits * pairs * s->units * p->rows_per_wave;
     s->partial_floats = splits > 1 ? part_rows * head_dim : 0;
     s->workspace = splits > 1 ? part_rows * (head_dim * 4 + 8) : 0;
-    if (splits > 1 && pairs * rows > 0x7fffffffl) return LUTGEMM_EINVAL;
     return LUTGEMM_OK;
 }
 
