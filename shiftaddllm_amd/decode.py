@@ -166,7 +166,7 @@ class LutDecoder(nn.Module):
             self.register_buffer("k_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
             self.register_buffer("v_cache", torch.zeros(shape, dtype=torch.float16, device=dev), persistent=False)
         else:
-            self.q4 = [Q4Cache(batch, cfg.kv_heads, cfg.max_positions, hd, dev) for _ in range(cfg.layers)]
+            self.q4 = nn.ModuleList(Q4Cache(batch, cfg.kv_heads, cfg.max_positions, hd, dev) for _ in range(cfg.layers))
             self.register_buffer("starts", torch.full((batch,), -1, dtype=torch.long, device=dev), persistent=False)
         if adapters is not None:
             self.register_buffer("adapter_ids", torch.full((batch,), -1, dtype=torch.int32, device=dev), persistent=False)

@@ -8,6 +8,7 @@ no counterpart: it decodes through the framework's fp16 cache (model/opt.py:367-
 from __future__ import annotations
 
 import torch
+import torch.nn as nn
 
 from . import native
 
@@ -15,11 +16,13 @@ GROUP = 32
 BLOCK = 32
 
 
-class Q4Cache:
+class Q4Cache(nn.Module):
     """Keys and values of `batch` sequences, `kv_heads` heads of `head_dim` numbers (a multiple of 32, at most 256), up to
-    `max_positions` positions.  `data` is the memory: uint8 [batch, kv_heads, blocks of 32 positions, 40 * head_dim], given or allocated."""
+    `max_positions` positions.  `data` is the memory: uint8 [batch, kv_heads, blocks of 32 positions, 40 * head_dim], given or allocated;
+    a buffer, so that a module's caches move with it, but none of its state."""
 
     def __init__(self, batch: int, kv_heads: int, max_positions: int, head_dim: int, device="cuda:0", data: torch.Tensor | None = None):
+        super().__init__()
         size = native.cabi().lutgemm_q4_cache_bytes(batch, kv_heads, max_positions, head_dim)
         if size == 0:
             raise ValueError(f"no 4-bit cache for batch={batch}, kv_heads={kv_heads}, max_positions={max_positions}, head_dim={head_dim} "
@@ -30,7 +33,7 @@ class Q4Cache:
             data = torch.zeros(shape, dtype=torch.uint8, device=device)
         if tuple(data.shape) != shape or data.dtype is not torch.uint8 or not data.is_contiguous():
             raise ValueError(f"data must be contiguous uint8 {shape}, is {data.dtype} {tuple(data.shape)}")
-        self.data = data
+        self.register_buffer("data", data, persistent=False)
 
     def attend(self, q, k, v, cos, sin, start, counts=None, out=None, held=False):
         """Appends the new tokens' keys (rotated) and values and returns attention over each sequence's positions up to each token.
@@ -40,7 +43,7 @@ class Q4Cache:
         new token, negative for an idle slot; counts int32 [batch]: how many of its tokens are there (None: all).  Tokens beyond the count or
         outside the cache are passed over, their rows are zeros.  With `held` also returns the values the cache holds for the
         new tokens' keys and values."""
-        return native.lutgemm.q4_attend(self.data, q, k, v, cos, sin, start, counts, out, held, self.max_positions)
+        return native.lutgemm.q4_attend(self._buffers["data"], q, k, v, cos, sin, start, counts, out, held, self.max_positions)
 
     def values(self, sequence: int, positions: int):
         """What the cache holds of the first `positions` positions of a sequence: keys and values, fp16 [positions, kv_heads, head_dim].
