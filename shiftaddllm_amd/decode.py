@@ -256,7 +256,7 @@ class LutDecoder(nn.Module):
 
     def _workspace(self, size):
         """Device memory for one call at a time of this decoder's stream.  (What was outgrown is kept: a captured step names it.)"""
-        if not self._workspaces or self._workspaces[-1].numel() < size:
+        if not self._workspaces or self._workspaces[-1].numel() < size or self._workspaces[-1].device != self.logits.device:
             self._workspaces.append(torch.empty(size, dtype=torch.uint8, device=self.logits.device))
         return self._workspaces[-1].data_ptr()
 

@@ -1,4 +1,4 @@
-"""A decoder's caches go where the decoder goes."""
+"""A decoder's caches and workspaces go where the decoder goes."""
 import torch
 
 from shiftaddllm_amd import decode
@@ -25,3 +25,12 @@ def test_a_cache_of_ones_own_is_the_memory_that_was_given():
     data = torch.zeros((1, 2, 2, 40 * 64), dtype=torch.uint8)
     cache = Q4Cache(1, 2, 40, 64, "cpu", data)
     assert cache.data is data and not cache.state_dict() and not list(cache.parameters())
+
+
+def test_workspaces_are_where_the_decoder_is():
+    m = decode.LutDecoder(CFG, None, device="cpu")
+    a = m._workspace(100)
+    assert m._workspace(50) == a
+    m.to("meta")
+    m._workspace(50)
+    assert m._workspaces[-1].device.type == "meta" and m._workspaces[0].device.type == "cpu"
