@@ -605,7 +605,8 @@ class LutDecoder(nn.Module):
     @torch.no_grad()
     def forward_token(self, ids: torch.Tensor, position):
         """One token per sequence at `position`; with a cache of 4 bits also a position for every sequence (a list or a tensor in
-        host memory), negative for one that is idle."""
+        host memory), negative for one that is idle: whatever its id is, and its logits mean nothing.  A decoder with sampling takes the id -1,
+        which a row of logits without weight gives, as token 0."""
         P = self.cfg.max_positions
         if not isinstance(position, (list, tuple)) and not (isinstance(position, torch.Tensor) and position.dim() > 0):
             # the attention kernel clamps the position into the cache: past its end it would
@@ -613,6 +614,7 @@ class LutDecoder(nn.Module):
             if not 0 <= position < P:
                 raise ValueError(f"position {position} outside the KV cache of {P} positions")
             (self.pos if self.kv_bits == 16 else self.starts).fill_(position)
+            positions = ()
         else:
             positions = [int(p) for p in position]
             if self.kv_bits != 4:
@@ -621,6 +623,11 @@ class LutDecoder(nn.Module):
                 raise ValueError(f"{self.batch} positions inside the KV cache of {P} positions are needed, got {positions}")
             self.starts.copy_(torch.tensor(positions))
         self.ids.copy_(ids)
+        # (the ids index the embedding: what stands for no token is no index)
+        if self.sampling is not None:
+            self.ids.clamp_(min=0)
+        if min(positions, default=0) < 0:
+            self.ids.masked_fill_(self.starts < 0, 0)
         if self._graph is not None:
             self._graph.replay()
         else:
