@@ -64,6 +64,8 @@ class DecoderConfig:
 
 LLAMA2_7B = DecoderConfig()
 
+PREFILL_ROWS = 65535   # tokens that prefill takes at once: rows of one quantised product
+
 
 def random_lut_linear(in_f, out_f, bits, group_size, gen, device):
     """LutLinear ("rowwise_fp16") with random sign planes and power-of-two scales
@@ -339,7 +341,7 @@ class LutDecoder(nn.Module):
     def prefill(self, input_ids: torch.Tensor, lengths=None, starts=None):
         """Takes prompts at once (cache of 4 bits): input_ids [batch, T], of which lengths[b] tokens are there (None: all), the first at
         position starts[b] (None: 0).  Leaves the logits behind each sequence's last token in self.logits and returns them; a
-        sequence without tokens keeps the logits that were there."""
+        sequence without tokens keeps the logits that were there.  More tokens than one product has rows (PREFILL_ROWS) are taken by parts."""
         if self.kv_bits != 4:
             raise ValueError("prefill needs a cache of 4 bits (kv_bits=4); the fp16 cache takes one token at a time")
         cfg, dev = self.cfg, self.logits.device
@@ -351,6 +353,11 @@ class LutDecoder(nn.Module):
         for n, p in zip(lengths, starts):
             if not 0 <= n <= T or (n > 0 and not 0 <= p <= cfg.max_positions - n):
                 raise ValueError(f"{n} tokens at position {p} outside the KV cache of {cfg.max_positions} positions")
+        most = PREFILL_ROWS // B
+        if T > most:
+            for t in range(0, T, most):
+                self.prefill(input_ids[:, t:t + most], [min(max(n - t, 0), most) for n in lengths], [p + t for p in starts])
+            return self.logits
         start = torch.tensor(starts, device=dev)
         count = torch.tensor(lengths, dtype=torch.int32, device=dev)
         ids = self.adapter_ids.repeat_interleave(T) if self.has_adapters else None
