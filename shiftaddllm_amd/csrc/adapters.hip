@@ -9,8 +9,8 @@
 //                       after the other.
 // A column of the instruction depends on nothing but its own row, so what rows stand beside it makes no difference to a result.
 // Bound by reading the adapters that are used (few rows), or x, base and out (many): 48 rows of 48 adapters of rank 64, 4096 to 11008, 95 MB
-// in 25.9 us (3.7 TB/s; a large copy 4.9); 4096 rows of 6 adapters of rank 32, 4096 to 4096, 44.4 us, of which sorting 6.9, the first
-// product 18.5, the second 18.5; one row 8.0 us, two launches in a row.  Up to 256 rows every workgroup finds by
+// in 26.0 us (3.7 TB/s; a large copy 4.9); 4096 rows of 6 adapters of rank 32, 4096 to 4096, 49.4 us (43.2 where x, base and out are the same ones
+// pass after pass), of which sorting 6.3 to 7.5, each product 18.5 to 19.6; one row 8.9 us, two launches in a row.  Up to 256 rows every workgroup finds by
 // itself which rows share its row's adapter; more rows are sorted by a launch ahead.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>

@@ -379,8 +379,8 @@ __device__ __forceinline__ f16x8 vector_of(const uint32_t (&w)[4]) { return __bu
 
 // Few query rows: the waves of a workgroup take the same 16 RT rows, and the blocks in turn, each block from memory to registers.
 // Bound by the stream of the cache: a wave holds a block at a time, the next one's keys are asked for when its scores are formed, its
-// values once they are folded in.  Two sequences of 131072 positions, 32 heads on 8 kv heads of 128: 336 MB in 68 us and 5 for the joining, 4.9 TB/s, as a large
-// copy on this card; vector instructions (366 a block, half of them the forming of held values) issue in 86 % of the cycles then.  64 sequences of 2048 positions 42 us, 4.0 TB/s.  One sequence at position 255 takes 9.2 us, of which an empty
+// values once they are folded in.  Two sequences of 131072 positions, 32 heads on 8 kv heads of 128: 336 MB in 67 us and 5 for the joining, 5.0 TB/s, as a large
+// copy on this card; vector instructions (365 a block, half of them the forming of held values) issue in 88 % of the cycles then.  64 sequences of 2048 positions 40 us, 4.2 TB/s.  One sequence at position 255 takes 8.9 us, of which an empty
 // launch is 2, the rest one block's way from memory through both products and the joining of four waves.
 template <int G, int RT>
 __global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attention_kernel(const Args a)
@@ -537,11 +537,11 @@ __global__ void __launch_bounds__(kThreads, G > 4 ? 1 : RT == 1 ? 3 : 2) attenti
 // itself does nothing else for most of its time (two prompts of 2048 tokens, 32 heads on 8: 197 us, vector unit 62 % busy, matrix unit 15 %).
 // Two buffers each, one barrier a block.  In the time of a block its weights are formed while the next block's scores are multiplied, from keys
 // that stand ready, and its values multiplied while the pieces of later blocks are formed; operands are read from LDS all at once, ahead of
-// their use (read one at a time, each wave waited for each: 107 us for those prompts).  Now 116 us, 14 of them appending: 560 TFLOP/s
+// their use (read one at a time, each wave waited for each: 107 us for those prompts without appending).  Now 114 us, 14 of them appending: 567 TFLOP/s
 // of the 1310 that a large fp16 product reaches.  Vector instructions (forming operands, weights, masks) issue in 55 % of the cycles, matrix
 // instructions run in 29 %; two waves per SIMD, which the registers of 32 rows of 128 dimensions allow, do not hide the rest.  Four waves instead of
 // eight form twice as much each: 140 us.  A third buffer of keys, read ahead of the barrier: 122 us.  A chunk of 256 tokens onto 30000
-// positions: 177 us, 715 TFLOP/s.
+// positions: 172 us, 737 TFLOP/s.
 template <int G>
 constexpr int kPromptTiles = G > 4 ? 1 : 2;   // tiles of 16 rows a wave takes, as registers allow
 

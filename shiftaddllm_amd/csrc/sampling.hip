@@ -6,10 +6,10 @@
 // which threads add; as many bits as leave room for the sum of a vocabulary, 43 (2^20 tokens) to 51.  A histogram of sums over steps of
 // a 64th of a power of two says in which step a target is reached; the few tokens of that step are then looked at one by one.  Where they are
 // many (equal logits, an endless temperature) digits of the logit's bits are followed instead.
-// Bound: 256 rows of 131072 fp32 logits, a CU each, 96 us: 23 us to read them for the largest (134 MB, 5.8 TB/s), 50 us for the weights (some
+// Bound: 256 rows of 131072 fp32 logits, a CU each, 94 us, of which (taken apart when it was 96) 23 us to read them for the largest (134 MB, 5.8 TB/s), 50 us for the weights (some
 // 25 instructions a logit 20 us, additions to the histogram in LDS 17 us, the list of the tokens near the largest 13 us), 22 us for the
 // choice, which reads a row again where the target is not among the listed tokens.  Few rows: three launches that wait for one another,
-// one row of 32000 with all filters 25.5 us (4, 7 and 14).
+// one row of 32000 with all filters 24.2 us (4, 7 and 14).
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
